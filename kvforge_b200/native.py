@@ -56,6 +56,10 @@ LIBRARIES: dict[str, tuple[list[str], list[str]]] = {
     "joint": (["joint_ops.cu"], []),
     # a matrix memory with exponential gates
     "memory": (["matrix_memory.cu"], []),
+    # several continuations of a prompt: which of them stay, and what of the cache and the states moves with them
+    "beams": (["beam_select.cu", "cache_copy.cu"], []),
+    # low-rank adapters of many requests at once
+    "adapters": (["adapters.cu"], []),
 }
 
 _loaded: dict[str, ctypes.CDLL] = {}

@@ -93,6 +93,14 @@ _SIGNATURES = {
     "kvf_memory_read_{s}": "plpplpfliiplp",
     "kvf_memory_columns": "i",
     "kvf_memory_set_pdl": "i",
+    # library "beams"
+    "kvf_beam_select_f32": "pliiiipppppp",
+    "kvf_copy_pages": "ppiipppiiiiiip",
+    "kvf_copy_states": "pilppiiip",
+    "kvf_beams_set_pdl": "i",
+    # library "adapters"
+    "kvf_adapter_add_{s}": "plppppp" + "i" * 6 + "i" * 4 + "plplipp",
+    "kvf_adapters_set_pdl": "i",
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 
@@ -175,7 +183,7 @@ def set_pdl(enabled: bool) -> None:
 _PDL_SETTERS = {
     "conv": "kvf_conv_set_pdl", "mixers": "kvf_mixers_set_pdl", "routed": "kvf_routed_set_pdl", "gated": "kvf_gated_set_pdl",
     "talking": "kvf_talking_set_pdl", "decay": "kvf_decay_set_pdl", "joint": "kvf_joint_set_pdl", "streams": "kvf_streams_set_pdl",
-    "memory": "kvf_memory_set_pdl",
+    "memory": "kvf_memory_set_pdl", "beams": "kvf_beams_set_pdl", "adapters": "kvf_adapters_set_pdl",
 }  # fmt: skip
 _library_pdl: dict[str, bool] = {}
 
@@ -2681,6 +2689,245 @@ def memory_read(o: torch.Tensor, floor: torch.Tensor, weight: torch.Tensor, eps:
         _fn(name, MEMORY_LIB)(
             _ptr(o), o.stride(0), _ptr(floor), _ptr(gate), gate.stride(0) if gate is not None else 0, _ptr(weight), float(eps), n, h, int(dv),
             _ptr(out), out.stride(0), _stream(),
+        ),
+        name,
+    )  # fmt: skip
+
+
+# ------------------------------------------------------------------ beams
+
+
+def _here(*tensors: torch.Tensor | None) -> None:
+    """Launches go to the current device's current stream: what they touch must live there."""
+    here = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("every operand must be a CUDA tensor (this engine has no CPU path)")
+        if here is None:
+            here = torch.cuda.current_device()
+        if t.get_device() != here:
+            raise ValueError(f"an operand lives on device {t.get_device()}, the current device is {here}")
+
+
+BEAM_MAX_K = 64  # candidates a prompt
+BEAM_MAX_WIDTH = 64  # beams a prompt
+
+
+def _beam_floats(rows: int, vocab: int, k: int) -> int:
+    return rows * (1 + k)
+
+
+def beam_workspace(rows: int, vocab: int, k: int, device: torch.device | str) -> torch.Tensor:
+    """What ``beam_select`` keeps between its stages for up to ``rows`` beams, ``vocab`` tokens and ``k`` candidates: int64,
+    zeros.  One call at a time uses it."""
+    if rows < 1 or vocab < 1 or not 1 <= k <= BEAM_MAX_K:
+        raise ValueError(f"beam_workspace: needs rows, a vocabulary and at most {BEAM_MAX_K} candidates")
+    return torch.zeros(_beam_floats(rows, vocab, k), dtype=torch.int64, device=device)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor, best: torch.Tensor, workspace: torch.Tensor) -> None:
+    """The best continuations of every prompt's beams: of ``scores[b] + log_softmax(logits[b])[t]`` over a prompt's beams and
+    the vocabulary the ``k`` highest, best first, of equal ones the lowest ``(b, t)``.
+
+    ``logits``: float ``[prompts * beams, V]``, a prompt's beams one after another; ``scores``: float, one a row.
+    ``parents`` (the beam's number within its prompt), ``tokens`` (int32) and ``best`` (float): ``[prompts, k]``.
+    A beam whose score is not finite, or whose logits hold a NaN, an infinity above or nothing above minus infinity, offers
+    nothing, nor does a token at minus infinity; places that nothing is left for get -1, -1 and minus infinity.
+    ``workspace``: ``beam_workspace`` for at least these sizes."""
+    if logits.dim() != 2 or parents.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
+        raise ValueError("beam_select: logits must be float [prompts * beams, V] with unit inner stride, parents [prompts, k]")
+    rows, v = logits.shape
+    prompts, k = parents.shape
+    if prompts < 1 or rows % prompts or rows < prompts or v < 1:
+        raise ValueError(f"beam_select: {rows} rows are not the beams of {prompts} prompts")
+    beams = rows // prompts
+    if beams > BEAM_MAX_WIDTH or not 1 <= k <= BEAM_MAX_K or beams * v > 2**31 - 1 or logits.stride(0) < v and rows > 1:
+        raise ValueError(f"beam_select: at most {BEAM_MAX_WIDTH} beams and {BEAM_MAX_K} candidates a prompt")
+    for t, dt, count, what in (
+        (scores, torch.float32, rows, "scores"), (parents, torch.int32, prompts * k, "parents"), (tokens, torch.int32, prompts * k, "tokens"),
+        (best, torch.float32, prompts * k, "best"), (workspace, torch.int64, 0, "workspace"),
+    ):  # fmt: skip
+        if t.dtype != dt or not t.is_contiguous() or (count and t.numel() != count):
+            raise ValueError(f"beam_select: {what} must be contiguous {dt}" + (f" with {count} entries" if count else ""))
+    if workspace.numel() < _beam_floats(rows, v, k):
+        raise ValueError("beam_select: the workspace is too small")
+    _here(logits, scores, parents, tokens, best, workspace)
+    name = "kvf_beam_select_f32"
+    _check(
+        _fn(name, "beams")(
+            _ptr(logits), logits.stride(0), prompts, beams, v, k, _ptr(scores), _ptr(workspace), _ptr(parents), _ptr(tokens), _ptr(best), _stream()
+        ),
+        name, 2,
+    )  # fmt: skip
+
+
+def _pairs(src: torch.Tensor, dst: torch.Tensor, what: str) -> int:
+    n = src.numel()
+    if src.dtype != torch.int32 or dst.dtype != torch.int32 or not src.is_contiguous() or not dst.is_contiguous() or dst.numel() != n:
+        raise ValueError(f"{what}: sources and targets are contiguous int32, one target a source")
+    return n
+
+
+def copy_pages(k: torch.Tensor, v: torch.Tensor | None, src: torch.Tensor, dst: torch.Tensor, tokens: torch.Tensor | None = None) -> None:
+    """Pages ``src[i]`` go to pages ``dst[i]`` in every layer: of ``k`` and ``v`` (``[entries, pages, heads, page size, head]``; ``v``
+    ``None`` where values lie inside the keys) the first ``tokens[i]`` positions, or the whole page.  Int32 lists; no target is a
+    source or another pair's target.  A pair with a page outside the pool copies nothing."""
+    n = _pairs(src, dst, "copy_pages")
+    if tokens is not None and (tokens.dtype != torch.int32 or not tokens.is_contiguous() or tokens.numel() != n):
+        raise ValueError("copy_pages: tokens are contiguous int32, one count a pair")
+    if k.dim() != 5 or not k.is_contiguous() or (v is not None and (v.shape[:4] != k.shape[:4] or v.dim() != 5 or v.dtype != k.dtype or not v.is_contiguous())):
+        raise ValueError("copy_pages: keys and values are contiguous [entries, pages, heads, page size, head] of one type")
+    entries, blocks, heads, bs, d = k.shape
+    size = k.element_size()
+    rows = (d * size, v.shape[4] * size if v is not None else 0)
+    if k.numel() == 0 or n == 0:
+        return
+    bits = rows[0] | rows[1] | k.data_ptr() | (v.data_ptr() if v is not None else 0)
+    unit = 16 if bits % 16 == 0 else 4 if bits % 4 == 0 else 2
+    if bits % 2 or entries > 65535:
+        raise ValueError("copy_pages: positions of an even number of bytes in at most 65,535 layers")
+    _here(k, v, src, dst, tokens)
+    name = "kvf_copy_pages"
+    _check(
+        _fn(name, "beams")(_ptr(k), _ptr(v), rows[0], rows[1], _ptr(src), _ptr(dst), _ptr(tokens), n, entries, blocks, heads, bs, unit, _stream()), name
+    )  # fmt: skip
+
+
+class StateTable:
+    """Where the recurrent states of a model lie: made once of its tensors ``[slots, ...]``, for ``copy_states``."""
+
+    def __init__(self, states: list[torch.Tensor]) -> None:
+        self.states = [t for t in states if t.numel()]
+        if not self.states:
+            raise ValueError("a table of states needs a state")
+        slots = {t.shape[0] for t in self.states}
+        if len(slots) != 1 or any(not t[0].is_contiguous() or t.device != self.states[0].device for t in self.states):
+            raise ValueError("states are [slots, ...] tensors of one device and one number of slots, each slot contiguous")
+        self.slots = slots.pop()
+        rows = [(t.data_ptr(), t.stride(0) * t.element_size(), t[0].numel() * t.element_size()) for t in self.states]
+        if any(stride < size and self.slots > 1 for _, stride, size in rows):
+            raise ValueError("the slots of a state overlap")
+        bits = 0
+        for row in rows:
+            bits |= row[0] | row[1] | row[2]
+        if bits % 4:
+            raise ValueError("states lie at multiples of four bytes")
+        self.unit = 16 if bits % 16 == 0 else 4
+        self.most = max(size for _, _, size in rows)
+        _here(*self.states)
+        self.rows = torch.tensor(rows, dtype=torch.int64, device=self.states[0].device)
+
+
+def copy_states(table: StateTable, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """The states in slots ``src[i]`` go to slots ``dst[i]`` in every tensor of the table.  Int32 lists; no target is a source or
+    another pair's target.  A pair with a slot outside the pool copies nothing."""
+    n = _pairs(src, dst, "copy_states")
+    if n == 0:
+        return
+    if n > 65535:
+        raise ValueError("copy_states: at most 65,535 copies a call")
+    _here(table.rows, src, dst)
+    name = "kvf_copy_states"
+    _check(_fn(name, "beams")(_ptr(table.rows), len(table.states), table.most, _ptr(src), _ptr(dst), n, table.slots, table.unit, _stream()), name)
+
+
+# ------------------------------------------------------------------ adapters
+
+
+ADAPTER_MAX_RANK = 128  # rows of a section
+ADAPTER_MAX_ROWS = 384  # rows of all sections
+ADAPTER_BLOCK = 8  # columns of a gate or an up in the alternating order
+
+
+class AdapterBank:
+    """The low-rank adapters of one projection, laid out once: ``a [S, sections, R, K]`` and ``b [S, N, R]`` in the storage type (float32
+    or bfloat16), ``scales`` float ``[S]``.  Adapter ``s`` adds ``scales[s] * b[s] (a[s] x)`` to the projection's result; a section is one of the
+    matrices that are stacked in the projection and has rows of ``a`` of its own.  ``ends``: the column after each section's last;
+    ``alternating``: two sections whose columns alternate in blocks of 8 (``interleave_gate_up``).  ``R`` is a multiple of 16: ranks
+    below it are filled with zeros; ``ranks`` (int32 ``[S]``) says how many rows of each section are not."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, ends=None, alternating: bool = False, ranks: torch.Tensor | None = None) -> None:
+        _suffix(a.dtype)
+        if a.dim() != 4 or b.dim() != 3 or b.dtype != a.dtype or not a.is_contiguous() or not b.is_contiguous():
+            raise ValueError("an adapter bank is contiguous a [S, sections, R, K] and b [S, N, R] of one type")
+        s, sections, r, k = a.shape
+        n = b.shape[1]
+        ends = (n,) if ends is None else tuple(int(e) for e in ends)
+        if s < 1 or b.shape[0] != s or b.shape[2] != r or len(ends) != sections:
+            raise ValueError("an adapter bank's a and b must agree in adapters, ranks and sections")
+        if r % 16 or not 0 < r <= ADAPTER_MAX_RANK or sections > 4 or sections * r > ADAPTER_MAX_ROWS:
+            raise ValueError(f"an adapter bank's rank is a multiple of 16 up to {ADAPTER_MAX_RANK}, {ADAPTER_MAX_ROWS} with all of at most four sections")
+        if k < 1 or n < 1 or k % 8 or n % 8 or any(e % 8 for e in ends):
+            raise ValueError("an adapter bank's widths and sections must be multiples of 8")
+        if list(ends) != sorted(set(ends)) or ends[0] <= 0 or ends[-1] != n:
+            raise ValueError("an adapter bank's sections end one after another, the last at its width")
+        if alternating and (sections != 2 or ends[0] * 2 != n):
+            raise ValueError("alternating sections are two of one width")
+        if scales.dtype != torch.float32 or scales.numel() != s or not scales.is_contiguous():
+            raise ValueError("an adapter bank has one float scale an adapter")
+        if ranks is not None and (ranks.dtype != torch.int32 or ranks.numel() != s or not ranks.is_contiguous()):
+            raise ValueError("an adapter bank has one int32 rank an adapter")
+        if a.data_ptr() % 16 or b.data_ptr() % 16:
+            raise ValueError("an adapter bank's matrices begin at multiples of 16 bytes")
+        if a.is_cuda and any(t is not None and t.device != a.device for t in (b, scales, ranks)):
+            raise ValueError("an adapter bank lives on one device")
+        self.a, self.b, self.scales, self.ranks = a, b, scales, ranks
+        self.ends, self.alternating = ends, bool(alternating)
+        self.size, self.sections, self.rank, self.k, self.n = s, sections, r, k, n
+
+
+class AdapterGroups:
+    """Which rows of a step take which adapter: made once for up to ``max_tokens`` rows and ``num_adapters`` adapters, filled by
+    ``group_by_adapter`` and read by every ``adapter_add`` of the step."""
+
+    def __init__(self, max_tokens: int, num_adapters: int, device: torch.device | str) -> None:
+        if max_tokens < 1 or num_adapters < 1:
+            raise ValueError("groups of adapters need room for a row and an adapter")
+        self.max_tokens, self.num_adapters = int(max_tokens), int(num_adapters)
+        self.device = torch.device(device)
+        self.ids: torch.Tensor | None = None
+        self.n = 0
+
+
+def group_by_adapter(ids: torch.Tensor, groups: AdapterGroups, err: torch.Tensor | None = None) -> None:
+    """Sort a step's rows by adapter: ``ids`` int32 ``[N]``, the adapter of every row or -1.  ``ids`` must stay as it is until
+    the step's last ``adapter_add``.  An id outside the bank counts as -1 and sets bit 32 of ``err``."""
+    if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous():
+        raise ValueError("group_by_adapter: ids are contiguous int32, one a row")
+    if ids.numel() > groups.max_tokens:
+        raise ValueError(f"group_by_adapter: {ids.numel()} rows, but the groups were made for {groups.max_tokens}")
+    _here(ids, err)
+    groups.ids, groups.n, groups.err = ids, ids.numel(), err
+
+
+def adapter_add(x: torch.Tensor, bank: AdapterBank, groups: AdapterGroups, out: torch.Tensor, base: torch.Tensor | None = None) -> None:
+    """``out[n] = base[n] + scales[s] * b[s] (a[s] x[n])`` with the adapter ``s`` of row ``n`` (``group_by_adapter``), and ``base[n]`` where that is
+    -1.  ``x [N, K]`` in the bank's type; ``out`` and ``base`` ``[N, width]`` in it or in float32.  ``base=None``: ``out`` is added to."""
+    s = _suffix(bank.a.dtype)
+    n, k = x.shape
+    if x.dtype != bank.a.dtype or k != bank.k or x.stride(1) != 1 or (x.stride(0) * x.element_size()) % 16 or x.data_ptr() % 16:
+        raise ValueError("adapter_add: x must be [N, K] of the bank's type and width, its rows at multiples of 16 bytes")
+    if groups.n != n or groups.ids is None or groups.num_adapters < bank.size:
+        raise ValueError("adapter_add: the groups are not those of these rows and this bank")
+    base = out if base is None else base
+    for t, what in ((out, "out"), (base, "base")):
+        if t.dtype not in (bank.a.dtype, torch.float32) or t.dtype != out.dtype or tuple(t.shape) != (n, bank.n):
+            raise ValueError(f"adapter_add: {what} must be [N, {bank.n}] of the bank's type or float32")
+        if t.stride(1) != 1 or (t.stride(0) * t.element_size()) % 16 or t.data_ptr() % 16:
+            raise ValueError(f"adapter_add: {what} needs unit inner stride and rows at multiples of 16 bytes")
+    if base is not out and base.data_ptr() == out.data_ptr() and base.stride(0) != out.stride(0):
+        raise ValueError("adapter_add: base and out overlap")
+    _here(x, bank.a, out, base, groups.ids)
+    if n == 0:
+        return
+    ends = (*bank.ends, bank.n, bank.n)
+    name = f"kvf_adapter_add_{s}"
+    _check(
+        _fn(name, "adapters")(
+            _ptr(x), x.stride(0), _ptr(bank.a), _ptr(bank.b), _ptr(bank.scales), _ptr(bank.ranks), _ptr(groups.ids), n, bank.size, bank.sections, bank.rank, k, bank.n,
+            ends[0], ends[1], ends[2], int(bank.alternating), _ptr(base), base.stride(0), _ptr(out), out.stride(0), int(out.dtype == torch.float32), _ptr(groups.err), _stream(),
         ),
         name,
     )  # fmt: skip
