@@ -94,7 +94,7 @@ _SIGNATURES = {
     "kvf_memory_columns": "i",
     "kvf_memory_set_pdl": "i",
     # library "beams"
-    "kvf_beam_select_f32": "pliiiipppppp",
+    "kvf_beam_select_f32": "pliiiipplpppp",
     "kvf_copy_pages": "ppiipppiiiiiip",
     "kvf_copy_states": "pilppiiip",
     "kvf_beams_set_pdl": "i",
@@ -2715,8 +2715,9 @@ BEAM_MAX_K = 64  # candidates a prompt
 BEAM_MAX_WIDTH = 64  # beams a prompt
 
 
-def _beam_floats(rows: int, vocab: int, k: int) -> int:
-    return rows * (1 + k)
+def _beam_words(rows: int, vocab: int, k: int) -> int:
+    """64-bit words of ``beam_select``'s records: K + 2 a stretch of at least 2,048 logits, K + 1 a row.  The records take the last three quarters of a workspace."""
+    return rows * (-(-vocab // 2048) * (k + 2) + k + 1)
 
 
 def beam_workspace(rows: int, vocab: int, k: int, device: torch.device | str) -> torch.Tensor:
@@ -2724,7 +2725,7 @@ def beam_workspace(rows: int, vocab: int, k: int, device: torch.device | str) ->
     zeros.  One call at a time uses it."""
     if rows < 1 or vocab < 1 or not 1 <= k <= BEAM_MAX_K:
         raise ValueError(f"beam_workspace: needs rows, a vocabulary and at most {BEAM_MAX_K} candidates")
-    return torch.zeros(_beam_floats(rows, vocab, k), dtype=torch.int64, device=device)
+    return torch.zeros(-(-4 * _beam_words(rows, vocab, k) // 3) + 4, dtype=torch.int64, device=device)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor, best: torch.Tensor, workspace: torch.Tensor) -> None:
@@ -2743,7 +2744,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tenso
     if prompts < 1 or rows % prompts or rows < prompts or v < 1:
         raise ValueError(f"beam_select: {rows} rows are not the beams of {prompts} prompts")
     beams = rows // prompts
-    if beams > BEAM_MAX_WIDTH or not 1 <= k <= BEAM_MAX_K or beams * v > 2**31 - 1 or logits.stride(0) < v and rows > 1:
+    if beams > BEAM_MAX_WIDTH or not 1 <= k <= BEAM_MAX_K or beams * v > 0x7FFF0000 or logits.stride(0) < v and rows > 1:
         raise ValueError(f"beam_select: at most {BEAM_MAX_WIDTH} beams and {BEAM_MAX_K} candidates a prompt")
     for t, dt, count, what in (
         (scores, torch.float32, rows, "scores"), (parents, torch.int32, prompts * k, "parents"), (tokens, torch.int32, prompts * k, "tokens"),
@@ -2751,15 +2752,16 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tenso
     ):  # fmt: skip
         if t.dtype != dt or not t.is_contiguous() or (count and t.numel() != count):
             raise ValueError(f"beam_select: {what} must be contiguous {dt}" + (f" with {count} entries" if count else ""))
-    if workspace.numel() < _beam_floats(rows, v, k):
+    words = workspace.numel()
+    if words - words // 4 < _beam_words(rows, v, k):
         raise ValueError("beam_select: the workspace is too small")
     _here(logits, scores, parents, tokens, best, workspace)
     name = "kvf_beam_select_f32"
     _check(
         _fn(name, "beams")(
-            _ptr(logits), logits.stride(0), prompts, beams, v, k, _ptr(scores), _ptr(workspace), _ptr(parents), _ptr(tokens), _ptr(best), _stream()
+            _ptr(logits), logits.stride(0), prompts, beams, v, k, _ptr(scores), _ptr(workspace), words, _ptr(parents), _ptr(tokens), _ptr(best), _stream()
         ),
-        name, 2,
+        name,
     )  # fmt: skip
 
 
