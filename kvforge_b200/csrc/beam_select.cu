@@ -3,14 +3,14 @@
 // A score that is no number (a row with a NaN, an infinity or nothing but masked tokens) and a beam whose own score is not
 // finite count as minus infinity; a place without a candidate above that gets parent and token -1.
 //
-// One pass over the logits, one launch.  A CTA holds a stretch of a row in registers (8 or 32 logits a thread) and leaves the
-// stretch's maximum, its sum of exponentials below that maximum and its K highest logits; the CTA that finishes a row's last
-// stretch does the same with the stretches' candidates, and the one that finishes a prompt's last row chooses among the rows'.
-// In each of the three steps the K highest are found without a sort: every warp's m-th highest thread maximum (m = K / 8 rounded
-// up) has at least K numbers of the CTA at or above the least of them, a bound that a few dozen numbers pass; those are gathered
-// and each counts the ones above it.  Where too many pass (rows of one value), the K highest are taken one after another.
-// Order is decided in 64 bits (a logit with its place; a score in double with its place), so equal numbers never depend on
-// which thread comes first; the sums of exponentials are joined in double in the order of the stretches.
+// One pass over the logits, one launch.  A CTA walks a stretch of a row, sixteen logits a thread at a time with the next sixteen on
+// their way, and leaves the stretch's maximum, its sum of exponentials below that maximum and its K highest logits; the CTA that
+// finishes a prompt's last stretch joins the sums and chooses among the stretches' candidates.
+// The K highest are found without a sort: every warp's m-th highest thread maximum (m = K / 8 rounded up) has at least K numbers of the CTA
+// at or above the least of the eight, a bound that rises as the walk goes on and that a few dozen numbers of a stretch pass; those are
+// gathered, and each counts the ones above it.  Where too many pass (rows of one value), the K highest are taken one after another.
+// Order is decided in 64 bits (a logit with its place; a score in double with its place), so equal numbers never depend on which
+// thread comes first; sums of sixteen exponentials are in float, all that joins them is in double and in one order.
 #include "common.cuh"
 
 using namespace kvf;
@@ -21,7 +21,9 @@ constexpr int MAX_K = 64;
 constexpr int MAX_W = 64;
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
-constexpr int CAP = 512;  // candidates that are ranked by counting
+constexpr int E = 16;               // logits a thread holds at a time
+constexpr int BATCH = THREADS * E;  // logits a CTA holds at a time
+constexpr int CAP = 768;            // candidates that are gathered
 
 typedef unsigned long long u64;
 
@@ -38,6 +40,11 @@ __device__ __forceinline__ double key_value64(u64 k) { return __longlong_as_doub
 // logit and place as one number, larger for a larger logit and, of equal ones, a lower place
 __device__ __forceinline__ u64 pack(float v, unsigned at) { return ((u64)ordered_key(v) << 32) | (0xffffffffu - at); }
 constexpr unsigned NOTHING = 0x007fffffu;  // ordered_key(-inf): what does not count
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 
 // A candidate: `hi`, then `lo`, the larger one first.
 struct Cand {
@@ -48,52 +55,70 @@ __device__ __forceinline__ bool above(const Cand& a, const Cand& b) { return a.h
 
 struct Shared {
   u64 hi[CAP];
+  u64 hi2[CAP];
   unsigned lo[CAP];
+  unsigned lo2[CAP];
   u64 out_hi[MAX_K];
   unsigned out_lo[MAX_K];
   unsigned least[WARPS];
   float warp_max[WARPS];
   double warp_sum[WARPS];
+  double lse[MAX_W];
   Cand round[WARPS];
-  int n, last, bad;
+  int n, n2, last;
 };
 
-// A bound that at least K of the CTA's numbers reach, if it holds that many (`top`: the thread's highest, ordered).
-__device__ __forceinline__ unsigned bound_of(unsigned top, int K, Shared& sh) {
-  const int m = (K + WARPS - 1) / WARPS;
+// The warp's m-th highest of its threads' numbers (not 0).
+__device__ __forceinline__ unsigned warp_mth(unsigned top, int m) {
   unsigned w = 0;
   for (int i = 0; i < m; ++i) {
     w = __reduce_max_sync(0xffffffffu, top);
-    const unsigned who = __ballot_sync(0xffffffffu, top == w);
-    if ((threadIdx.x & 31) == __ffs(who) - 1) top = 0;
+    if (i + 1 < m) {
+      const unsigned who = __ballot_sync(0xffffffffu, top == w);
+      if ((threadIdx.x & 31) == __ffs(who) - 1) top = 0;
+    }
   }
-  if ((threadIdx.x & 31) == 0) sh.least[threadIdx.x >> 5] = w;
-  if (threadIdx.x == 0) sh.n = 0;
-  __syncthreads();
-  unsigned least = sh.least[0];
+  return w;
+}
+// The least of what the warps have posted; they post numbers that rise, so one posted before is a bound too.
+__device__ __forceinline__ unsigned posted_bound(const Shared& sh) {
+  const volatile unsigned* l = sh.least;
+  unsigned least = l[0];
 #pragma unroll
-  for (int i = 1; i < WARPS; ++i) least = min(least, sh.least[i]);
+  for (int i = 1; i < WARPS; ++i) least = min(least, (unsigned)l[i]);
   return max(least, NOTHING + 1);
 }
+__device__ __forceinline__ void put(const Cand& c, Shared& sh) {
+  const int at = atomicAdd(&sh.n, 1);
+  if (at < CAP) {
+    sh.hi[at] = c.hi;
+    sh.lo[at] = c.lo;
+  }
+}
 
-// The K highest of what `each(f)` hands to f(candidate) on every thread, into out_hi / out_lo, best first; returns how many there are.
-// `gather(put)`: calls put(candidate) for those at or above the bound.
-template <class Gather, class Each>
-__device__ __forceinline__ int k_highest(int K, Shared& sh, Gather gather, Each each) {
-  gather([&](const Cand& c) {
-    const int at = atomicAdd(&sh.n, 1);
-    if (at < CAP) {
-      sh.hi[at] = c.hi;
-      sh.lo[at] = c.lo;
-    }
-  });
+// The K highest of what was put (all of those at or above `bound`, a number of `key`), into out_hi / out_lo, best first; returns how many
+// there are.  `each(f)` hands every number there is to f, for when more were put than there is room for.  Begins and ends with a barrier.
+template <class Key, class Each>
+__device__ __forceinline__ int k_highest(int K, Shared& sh, unsigned bound, Key key, Each each) {
+  if (threadIdx.x == 0) sh.n2 = 0;
   __syncthreads();
-  const int n = sh.n;
+  int n = sh.n;
   if (n <= CAP) {
+    // the bound rose after some had been put
     for (int i = threadIdx.x; i < n; i += THREADS) {
-      const Cand c{sh.hi[i], sh.lo[i]};
+      if (key(sh.hi[i]) >= bound) {
+        const int at = atomicAdd(&sh.n2, 1);
+        sh.hi2[at] = sh.hi[i];
+        sh.lo2[at] = sh.lo[i];
+      }
+    }
+    __syncthreads();
+    n = sh.n2;
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+      const Cand c{sh.hi2[i], sh.lo2[i]};
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += above(Cand{sh.hi[j], sh.lo[j]}, c);
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) rank += above(Cand{sh.hi2[j], sh.lo2[j]}, c);
       if (rank < K) {
         sh.out_hi[rank] = c.hi;
         sh.out_lo[rank] = c.lo;
@@ -133,211 +158,210 @@ struct BeamParams {
   const float* logits;
   long long stride;
   const float* scores;
-  int prompts, W, V, K, stretches;
-  int* tickets;    // [rows] stretches done, [prompts] rows done: zeros between calls
-  double* sums;    // [rows][stretches]
-  float* maxima;   // [rows][stretches]
-  u64* cands;      // [rows][stretches][K]
-  double* lse;     // [rows]
-  u64* row_cands;  // [rows][K]
+  int prompts, W, V, K;
+  int batches;    // of a stretch
+  int stretches;  // of a row
+  int* tickets;   // [prompts] stretches done: zeros between calls
+  double* sums;   // [rows][stretches]
+  float* maxima;  // [rows][stretches]
+  u64* cands;     // [rows][stretches][K]
   int* parents;
   int* tokens;
   float* best;
 };
 
-// Whether this CTA is the last of `of` that come here; what the others wrote before is then visible.
-__device__ __forceinline__ bool last_of(int* ticket, int of, Shared& sh) {
-  if (of == 1) {
-    __syncthreads();
-    return true;
+template <bool VEC>
+__device__ __forceinline__ int place(int first, int e) { return first + (VEC ? 4 * threadIdx.x + (e >> 2) * (4 * THREADS) + (e & 3) : threadIdx.x + e * THREADS); }
+
+template <bool VEC>
+__device__ __forceinline__ void load_batch(float (&v)[E], const float* x, int first, int V) {
+  if (VEC) {
+#pragma unroll
+    for (int q = 0; q < E / 4; ++q) {
+      const int i = place<VEC>(first, 4 * q);
+      if (i + 4 <= V) {
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i));
+        v[4 * q] = f.x, v[4 * q + 1] = f.y, v[4 * q + 2] = f.z, v[4 * q + 3] = f.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * q + e] = i + e < V ? __ldcs(x + i + e) : -INFINITY;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = place<VEC>(first, e) < V ? __ldcs(x + place<VEC>(first, e)) : -INFINITY;
   }
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const int t = atomicAdd(ticket, 1);
-    sh.last = t == of - 1;
-    if (sh.last) *ticket = 0;
-  }
-  __syncthreads();
-  if (sh.last) __threadfence();
-  return sh.last;
 }
 
 // VEC: rows begin at multiples of 16 bytes, four logits a load.  All rows of a call are dealt out to threads alike, so that equal rows have
 // equal sums and their candidates are ties.
-template <int E, bool VEC>
-__global__ void __launch_bounds__(THREADS, E > 16 ? 3 : 4) beam_select_kernel(BeamParams p) {
+template <bool VEC>
+__global__ void __launch_bounds__(THREADS, 4) beam_select_kernel(BeamParams p) {
   pdl_launch();
   __shared__ Shared sh;
   const int row = blockIdx.x / p.stretches, stretch = blockIdx.x - row * p.stretches;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float* x = p.logits + (long long)row * p.stride;
-  const int K = p.K;
-  float v[E];
-  const int first = stretch * (THREADS * E) + (VEC ? 4 : 1) * threadIdx.x;
-  const auto place = [&](int e) { return first + (VEC ? (e >> 2) * (4 * THREADS) + (e & 3) : e * THREADS); };
+  const int K = p.K, V = p.V, mth = (K + WARPS - 1) / WARPS;
+  const int first = stretch * p.batches * BATCH;
+  const int batches = min(p.batches, (V - first + BATCH - 1) / BATCH);
+  if (threadIdx.x == 0) sh.n = 0;
+  constexpr float L2E = 1.4426950408889634f, L2E_LOW = (float)(1.4426950408889634 - (double)L2E);
+  float v[E], next[E];
+  float high = -INFINITY, m = -INFINITY, s = 0.f;  // the thread's highest logit; the warp's, and the thread's sum of exponentials below it
   pdl_wait();
-  if (VEC) {
+  load_batch<VEC>(v, x, first, V);
+  for (int b = 0; b < batches; ++b) {
+    const int at = first + b * BATCH;
+    if (b + 1 < batches) load_batch<VEC>(next, x, at + BATCH, V);
+    float top = v[0];
 #pragma unroll
-    for (int q = 0; q < E / 4; ++q) {
-      const int i = place(4 * q);
-      if (i + 4 <= p.V) {
-        const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i));
-        v[4 * q] = f.x, v[4 * q + 1] = f.y, v[4 * q + 2] = f.z, v[4 * q + 3] = f.w;
-      } else {
+    for (int e = 1; e < E; ++e) top = fmaxf(top, v[e]);  // (a NaN is passed over here and shows in the sum)
+    top = fmaxf(top, -INFINITY);
+    high = fmaxf(high, top);
+    const unsigned key = ordered_key(high);
+    const float wm = key_value(__reduce_max_sync(0xffffffffu, key));
+    const unsigned w = warp_mth(key, mth);
+    if (lane == 0) *(volatile unsigned*)&sh.least[warp] = w;
+    if (b == 0) __syncthreads();
+    const float least = key_value(posted_bound(sh));
+    if (top >= least) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * q + e] = i + e < p.V ? __ldcs(x + i + e) : -INFINITY;
-      }
+      for (int e = 0; e < E; ++e)
+        if (v[e] >= least) put(Cand{pack(v[e], place<VEC>(at, e)), 0}, sh);
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = place(e) < p.V ? __ldcs(x + place(e)) : -INFINITY;
-  }
-  float top = v[0];
-  bool bad = false;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    top = fmaxf(top, v[e]);
-    bad |= isnan(v[e]);
-  }
-  if (isnan(top)) top = -INFINITY;
-  {
-    const float w = warp_max(top);
-    if (lane == 0) sh.warp_max[warp] = w;
-  }
-  const unsigned bound = bound_of(ordered_key(top), K, sh);  // (a barrier lies in it)
-  float m = sh.warp_max[0];
-#pragma unroll
-  for (int i = 1; i < WARPS; ++i) m = fmaxf(m, sh.warp_max[i]);
-  const float least = key_value(bound);
-  {
-    // a stretch with nothing in it has no sum; a NaN or an infinity leaves NaN
-    float s = 0.f;
-    if (m > -INFINITY) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) s += expf(v[e] - m);
+    if (wm > m) {
+      s *= ex2((m - wm) * L2E);
+      m = wm;
     }
-    if (bad) s = NAN;
+    const float below = m > -INFINITY ? m : 0.f;
+    float part = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float d = v[e] - below;  // exact for the logits that weigh most
+      part += ex2(fmaf(d, L2E, d * L2E_LOW));
+    }
+    s += part;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = next[e];
+  }
+  {
     double d = s;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (lane == 0) sh.warp_sum[warp] = d;
+    if (lane == 0) {
+      sh.warp_max[warp] = m;
+      sh.warp_sum[warp] = d;
+    }
   }
-  const int found = k_highest(
-      K, sh,
-      [&](auto put) {
-        if (top >= least) {
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (v[e] >= least) put(Cand{pack(v[e], place(e)), 0});
-        }
-      },
-      [&](auto see) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (v[e] > -INFINITY) see(Cand{pack(v[e], place(e)), 0});
-      });
+  __syncthreads();
   const long long rec = (long long)row * p.stretches + stretch;
+  const int found = k_highest(
+      K, sh, posted_bound(sh), [](u64 hi) { return (unsigned)(hi >> 32); },
+      [&](auto see) {
+        for (int i = first + threadIdx.x; i < min(V, first + batches * BATCH); i += THREADS)
+          if (x[i] > -INFINITY) see(Cand{pack(x[i], i), 0});
+      });
   for (int k = threadIdx.x; k < K; k += THREADS) p.cands[rec * K + k] = k < found ? sh.out_hi[k] : 0;
-  if (threadIdx.x == 0) {
-    double s = 0;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) s += sh.warp_sum[i];
-    p.sums[rec] = s;
-    p.maxima[rec] = m;
-  }
-  if (!last_of(p.tickets + row, p.stretches, sh)) return;
-
-  // ---- the row: its logarithm of the sum, and the K highest of the stretches' candidates
-  const long long rec0 = (long long)row * p.stretches;
-  {
-    float rm = -INFINITY;
-    for (int i = threadIdx.x; i < p.stretches; i += THREADS) rm = fmaxf(rm, __ldcg(p.maxima + rec0 + i));
-    rm = warp_max(rm);
-    if (lane == 0) sh.warp_max[warp] = rm;
-    __syncthreads();
-    rm = sh.warp_max[0];
-#pragma unroll
-    for (int i = 1; i < WARPS; ++i) rm = fmaxf(rm, sh.warp_max[i]);
-    double s = 0;
-    for (int i = threadIdx.x; i < p.stretches; i += THREADS) {
-      const float sm = __ldcg(p.maxima + rec0 + i);
-      const double part = __ldcg(p.sums + rec0 + i);
-      if (sm > -INFINITY || isnan(part)) s += part * exp((double)sm - (double)rm);
+  if (warp == 1) {
+    float hi = lane < WARPS ? sh.warp_max[lane] : -INFINITY;
+    const float all = warp_max(hi);
+    double d = 0;
+    if (lane < WARPS) {
+      d = sh.warp_sum[lane];
+      if (hi > -INFINITY) d *= exp((double)hi - (double)all);
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) sh.warp_sum[warp] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      double t = 0;
-#pragma unroll
-      for (int i = 0; i < WARPS; ++i) t += sh.warp_sum[i];
-      p.lse[row] = isinf(rm) ? (double)NAN : (double)rm + log(t);
+    for (int o = 4; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (lane == 0) {
+      p.sums[rec] = d;
+      p.maxima[rec] = all;
     }
   }
-  const u64* cands = p.cands + rec0 * K;
-  const int total = p.stretches * K;
-  unsigned high = 0;
-  for (int i = threadIdx.x; i < total; i += THREADS) high = max(high, (unsigned)(__ldcg(cands + i) >> 32));
-  const unsigned row_bound = bound_of(high, K, sh);
-  const int row_found = k_highest(
-      K, sh,
-      [&](auto put) {
-        for (int i = threadIdx.x; i < total; i += THREADS) {
-          const u64 c = __ldcg(cands + i);
-          if ((unsigned)(c >> 32) >= row_bound) put(Cand{c, 0});
-        }
-      },
-      [&](auto see) {
-        for (int i = threadIdx.x; i < total; i += THREADS) {
-          const u64 c = __ldcg(cands + i);
-          if (c) see(Cand{c, 0});
-        }
-      });
-  for (int k = threadIdx.x; k < K; k += THREADS) p.row_cands[(long long)row * K + k] = k < row_found ? sh.out_hi[k] : 0;
   const int prompt = row / p.W, row0 = prompt * p.W;
-  if (!last_of(p.tickets + p.prompts * p.W + prompt, p.W, sh)) return;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    // what the CTA wrote is seen by whoever sees its ticket
+    __threadfence();
+    const int t = atomicAdd(p.tickets + prompt, 1);
+    sh.last = t == p.W * p.stretches - 1;
+    if (sh.last) {
+      p.tickets[prompt] = 0;
+      __threadfence();
+    }
+    sh.n = 0;
+  }
+  __syncthreads();
+  if (!sh.last) return;
 
-  // ---- the prompt: scores in double; the bound goes by the scores rounded to floats (a rounding keeps the order)
-  const int all = p.W * K;
+  // ---- the prompt: the rows' logarithms of the sums, a warp a row
+  for (int b = warp; b < p.W; b += WARPS) {
+    const long long r0 = (long long)(row0 + b) * p.stretches;
+    float all = -INFINITY;
+    for (int i = lane; i < p.stretches; i += 32) all = fmaxf(all, __ldcg(p.maxima + r0 + i));
+    all = warp_max(all);
+    double d = 0;
+    for (int i = lane; i < p.stretches; i += 32) {
+      const float hi = __ldcg(p.maxima + r0 + i);
+      const double part = __ldcg(p.sums + r0 + i);
+      if (hi > -INFINITY || isnan(part)) d += part * exp((double)hi - (double)all);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (lane == 0) sh.lse[b] = isinf(all) ? (double)NAN : (double)all + log(d);
+  }
+  __syncthreads();
+  // ---- the K highest of the stretches' candidates: scores in double; the bound goes by the scores rounded to floats (a rounding keeps the order)
+  const int each_row = p.stretches * K, every = p.W * each_row;
+  const u64* cands = p.cands + (long long)row0 * each_row;
   auto candidate = [&](int i) {
-    const int b = i / K;
-    const u64 c = __ldcg(p.row_cands + (long long)row0 * K + i);
+    const int b = i / each_row;
+    const u64 c = __ldcg(cands + i);
     const float own = __ldg(p.scores + row0 + b);
-    double s = (double)own + ((double)key_value((unsigned)(c >> 32)) - __ldcg(p.lse + row0 + b));
-    if (c == 0 || isnan(s) || !isfinite(own) || (float)s == -INFINITY) s = -INFINITY;
-    return Cand{ordered_key64(s), 0xffffffffu - ((unsigned)b * p.V + (0xffffffffu - (unsigned)c))};
+    double sc = (double)own + ((double)key_value((unsigned)(c >> 32)) - sh.lse[b]);
+    if (c == 0 || isnan(sc) || !isfinite(own) || (float)sc == -INFINITY) sc = -INFINITY;
+    return Cand{ordered_key64(sc), 0xffffffffu - ((unsigned)b * V + (0xffffffffu - (unsigned)c))};
   };
-  unsigned score = 0;
-  for (int i = threadIdx.x; i < all; i += THREADS) score = max(score, ordered_key((float)key_value64(candidate(i).hi)));
-  const unsigned prompt_bound = bound_of(score, K, sh);
-  const int chosen = k_highest(
-      K, sh,
-      [&](auto put) {
-        for (int i = threadIdx.x; i < all; i += THREADS) {
-          const Cand c = candidate(i);
-          if (ordered_key((float)key_value64(c.hi)) >= prompt_bound) put(c);
-        }
-      },
-      [&](auto see) {
-        for (int i = threadIdx.x; i < all; i += THREADS) {
-          const Cand c = candidate(i);
-          if (key_value64(c.hi) > -INFINITY) see(c);
-        }
-      });
+  auto score_key = [](u64 hi) { return ordered_key((float)key_value64(hi)); };
+  unsigned top = 0;
+  for (int i = threadIdx.x; i < every; i += THREADS) top = max(top, score_key(candidate(i).hi));
+  const unsigned w = warp_mth(top, mth);
+  if (lane == 0) sh.least[warp] = w;
+  __syncthreads();
+  const unsigned bound = posted_bound(sh);
+  for (int i = threadIdx.x; i < every; i += THREADS) {
+    const Cand c = candidate(i);
+    if (score_key(c.hi) >= bound) put(c, sh);
+  }
+  const int chosen = k_highest(K, sh, bound, score_key, [&](auto see) {
+    for (int i = threadIdx.x; i < every; i += THREADS) {
+      const Cand c = candidate(i);
+      if (key_value64(c.hi) > -INFINITY) see(c);
+    }
+  });
   for (int k = threadIdx.x; k < K; k += THREADS) {
     const bool none = k >= chosen || sh.out_hi[k] == 0;
     const unsigned at = 0xffffffffu - sh.out_lo[k];
-    p.parents[prompt * K + k] = none ? -1 : (int)(at / p.V);
-    p.tokens[prompt * K + k] = none ? -1 : (int)(at % p.V);
+    p.parents[prompt * K + k] = none ? -1 : (int)(at / V);
+    p.tokens[prompt * K + k] = none ? -1 : (int)(at % V);
     p.best[prompt * K + k] = none ? -INFINITY : (float)key_value64(sh.out_hi[k]);
   }
 }
 
-// Logits a CTA: 32 a thread where that still makes four CTAs for every SM (three are on one at a time), else 8.
-int stretches_of(int V, int per) { return (V + THREADS * per - 1) / (THREADS * per); }
-int per_thread(long long rows, int V) { return rows * stretches_of(V, 32) >= 4 * 148 ? 32 : 8; }
+// Batches a CTA walks: CTAs run four to an SM, each costs about two batches besides those it walks, and what counts is the number of
+// times the device fills up with them.
+int batches_of(long long rows, int V) {
+  const int all = (V + BATCH - 1) / BATCH;
+  int best = 1;
+  long long least = -1;
+  for (int b = 1; b <= all; ++b) {
+    const long long ctas = rows * ((all + b - 1) / b);
+    const long long cost = ((ctas + 4 * 148 - 1) / (4 * 148)) * (b + 2);
+    if (least < 0 || cost < least) least = cost, best = b;
+    if (b > 64) break;
+  }
+  return best;
+}
 
 }  // namespace
 
@@ -347,28 +371,26 @@ KVF_API int kvf_beams_set_pdl(int on) {
 }
 
 // work: `words` eight-byte words; the first quarter holds the tickets, zeros between calls, whatever the sizes of a call.  The rest takes
-// the records: K + 2 words a stretch (of at least 2,048 logits) and K + 1 a row.
+// the records: K + 2 words a stretch (of at least 4,096 logits).
 KVF_API int kvf_beam_select_f32(const float* logits, long long stride, int prompts, int W, int V, int K, const float* scores, void* work, long long words, int* parents,
                                 int* tokens, float* best, cudaStream_t st) {
   if (prompts <= 0) return 0;
   const long long rows = (long long)prompts * W;
   if (W < 1 || W > MAX_W || K < 1 || K > MAX_K || V < 1 || (long long)W * V > 0x7fff0000ll) return (int)cudaErrorInvalidValue;
-  const int per = per_thread(rows, V), s = stretches_of(V, per);
-  const long long quarter = words / 4;
-  if (rows > quarter || rows * (s * (K + 2ll) + K + 1) > words - quarter || rows * s > 0x7fffffffll) return (int)cudaErrorInvalidValue;
   BeamParams p;
+  p.batches = batches_of(rows, V);
+  p.stretches = ((V + BATCH - 1) / BATCH + p.batches - 1) / p.batches;
+  const long long quarter = words / 4, records = rows * p.stretches;
+  if (prompts > 2 * quarter || records * (K + 2) > words - quarter || records > 0x7fffffffll) return (int)cudaErrorInvalidValue;
   p.logits = logits, p.stride = stride, p.scores = scores;
-  p.prompts = prompts, p.W = W, p.V = V, p.K = K, p.stretches = s;
+  p.prompts = prompts, p.W = W, p.V = V, p.K = K;
   p.tickets = reinterpret_cast<int*>(work);
   u64* at = reinterpret_cast<u64*>(work) + quarter;
-  p.cands = at, at += rows * s * K;
-  p.row_cands = at, at += rows * K;
-  p.sums = reinterpret_cast<double*>(at), at += rows * s;
-  p.lse = reinterpret_cast<double*>(at), at += rows;
+  p.cands = at, at += records * K;
+  p.sums = reinterpret_cast<double*>(at), at += records;
   p.maxima = reinterpret_cast<float*>(at);
   p.parents = parents, p.tokens = tokens, p.best = best;
-  const dim3 grid((unsigned)(rows * s)), block(THREADS);
+  const dim3 grid((unsigned)records), block(THREADS);
   const bool vec = stride % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
-  if (per == 32) return vec ? launch(beam_select_kernel<32, true>, grid, block, 0, st, p) : launch(beam_select_kernel<32, false>, grid, block, 0, st, p);
-  return vec ? launch(beam_select_kernel<8, true>, grid, block, 0, st, p) : launch(beam_select_kernel<8, false>, grid, block, 0, st, p);
+  return vec ? launch(beam_select_kernel<true>, grid, block, 0, st, p) : launch(beam_select_kernel<false>, grid, block, 0, st, p);
 }

@@ -2716,8 +2716,8 @@ BEAM_MAX_WIDTH = 64  # beams a prompt
 
 
 def _beam_words(rows: int, vocab: int, k: int) -> int:
-    """64-bit words of ``beam_select``'s records: K + 2 a stretch of at least 2,048 logits, K + 1 a row.  The records take the last three quarters of a workspace."""
-    return rows * (-(-vocab // 2048) * (k + 2) + k + 1)
+    """64-bit words of ``beam_select``'s records: K + 2 a stretch of at least 4,096 logits.  The records take the last three quarters of a workspace."""
+    return rows * -(-vocab // 4096) * (k + 2)
 
 
 def beam_workspace(rows: int, vocab: int, k: int, device: torch.device | str) -> torch.Tensor:
