@@ -51,7 +51,7 @@ struct Cand {
   u64 hi;
   unsigned lo;
 };
-__device__ __forceinline__ bool above(const Cand& a, const Cand& b) { return a.hi > b.hi || (a.hi == b.hi && a.lo > b.lo); }
+__device__ __forceinline__ int above(const Cand& a, const Cand& b) { return (a.hi > b.hi) | ((a.hi == b.hi) & (a.lo > b.lo)); }  // (without a branch)
 
 struct Shared {
   u64 hi[CAP];
@@ -88,17 +88,19 @@ __device__ __forceinline__ unsigned posted_bound(const Shared& sh) {
   for (int i = 1; i < WARPS; ++i) least = min(least, (unsigned)l[i]);
   return max(least, NOTHING + 1);
 }
+template <bool LO>
 __device__ __forceinline__ void put(const Cand& c, Shared& sh) {
   const int at = atomicAdd(&sh.n, 1);
   if (at < CAP) {
     sh.hi[at] = c.hi;
-    sh.lo[at] = c.lo;
+    if (LO) sh.lo[at] = c.lo;
   }
 }
 
 // The K highest of what was put (all of those at or above `bound`, a number of `key`), into out_hi / out_lo, best first; returns how many
 // there are.  `each(f)` hands every number there is to f, for when more were put than there is room for.  Begins and ends with a barrier.
-template <class Key, class Each>
+// LO: `lo` differs between candidates of equal `hi` (else there are none).
+template <bool LO, class Key, class Each>
 __device__ __forceinline__ int k_highest(int K, Shared& sh, unsigned bound, Key key, Each each) {
   if (threadIdx.x == 0) sh.n2 = 0;
   __syncthreads();
@@ -109,19 +111,19 @@ __device__ __forceinline__ int k_highest(int K, Shared& sh, unsigned bound, Key 
       if (key(sh.hi[i]) >= bound) {
         const int at = atomicAdd(&sh.n2, 1);
         sh.hi2[at] = sh.hi[i];
-        sh.lo2[at] = sh.lo[i];
+        if (LO) sh.lo2[at] = sh.lo[i];
       }
     }
     __syncthreads();
     n = sh.n2;
     for (int i = threadIdx.x; i < n; i += THREADS) {
-      const Cand c{sh.hi2[i], sh.lo2[i]};
+      const Cand c{sh.hi2[i], LO ? sh.lo2[i] : 0};
       int rank = 0;
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) rank += above(Cand{sh.hi2[j], sh.lo2[j]}, c);
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) rank += LO ? above(Cand{sh.hi2[j], sh.lo2[j]}, c) : (int)(sh.hi2[j] > c.hi);
       if (rank < K) {
         sh.out_hi[rank] = c.hi;
-        sh.out_lo[rank] = c.lo;
+        if (LO) sh.out_lo[rank] = c.lo;
       }
     }
     __syncthreads();
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, 4) beam_select_kernel(BeamParams p) {
     if (top >= least) {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (v[e] >= least) put(Cand{pack(v[e], place<VEC>(at, e)), 0}, sh);
+        if (v[e] >= least) put<false>(Cand{pack(v[e], place<VEC>(at, e)), 0}, sh);
     }
     if (wm > m) {
       s *= ex2((m - wm) * L2E);
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(THREADS, 4) beam_select_kernel(BeamParams p) {
   }
   __syncthreads();
   const long long rec = (long long)row * p.stretches + stretch;
-  const int found = k_highest(
+  const int found = k_highest<false>(
       K, sh, posted_bound(sh), [](u64 hi) { return (unsigned)(hi >> 32); },
       [&](auto see) {
         for (int i = first + threadIdx.x; i < min(V, first + batches * BATCH); i += THREADS)
@@ -269,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, 4) beam_select_kernel(BeamParams p) {
     double d = 0;
     if (lane < WARPS) {
       d = sh.warp_sum[lane];
-      if (hi > -INFINITY) d *= exp((double)hi - (double)all);
+      if (hi > -INFINITY) d *= (double)expf(hi - all);
     }
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
@@ -282,13 +284,10 @@ __global__ void __launch_bounds__(THREADS, 4) beam_select_kernel(BeamParams p) {
   __syncthreads();
   if (threadIdx.x == 0) {
     // what the CTA wrote is seen by whoever sees its ticket
-    __threadfence();
-    const int t = atomicAdd(p.tickets + prompt, 1);
+    int t;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(t) : "l"(p.tickets + prompt) : "memory");
     sh.last = t == p.W * p.stretches - 1;
-    if (sh.last) {
-      p.tickets[prompt] = 0;
-      __threadfence();
-    }
+    if (sh.last) p.tickets[prompt] = 0;
     sh.n = 0;
   }
   __syncthreads();
@@ -297,15 +296,18 @@ __global__ void __launch_bounds__(THREADS, 4) beam_select_kernel(BeamParams p) {
   // ---- the prompt: the rows' logarithms of the sums, a warp a row
   for (int b = warp; b < p.W; b += WARPS) {
     const long long r0 = (long long)(row0 + b) * p.stretches;
-    float all = -INFINITY;
-    for (int i = lane; i < p.stretches; i += 32) all = fmaxf(all, __ldcg(p.maxima + r0 + i));
-    all = warp_max(all);
+    // (a lane joins its stretches one after another: one each up to 32 stretches)
+    float hi = -INFINITY;
     double d = 0;
     for (int i = lane; i < p.stretches; i += 32) {
-      const float hi = __ldcg(p.maxima + r0 + i);
+      const float next = __ldcg(p.maxima + r0 + i);
       const double part = __ldcg(p.sums + r0 + i);
-      if (hi > -INFINITY || isnan(part)) d += part * exp((double)hi - (double)all);
+      const float both = fmaxf(hi, next);
+      if (both > -INFINITY || isnan(part)) d = d * (double)expf(hi - both) + part * (double)expf(next - both);
+      hi = both;
     }
+    const float all = warp_max(hi);
+    if (hi > -INFINITY) d *= (double)expf(hi - all);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
     if (lane == 0) sh.lse[b] = isinf(all) ? (double)NAN : (double)all + log(d);
@@ -324,16 +326,23 @@ __global__ void __launch_bounds__(THREADS, 4) beam_select_kernel(BeamParams p) {
   };
   auto score_key = [](u64 hi) { return ordered_key((float)key_value64(hi)); };
   unsigned top = 0;
-  for (int i = threadIdx.x; i < every; i += THREADS) top = max(top, score_key(candidate(i).hi));
-  const unsigned w = warp_mth(top, mth);
-  if (lane == 0) sh.least[warp] = w;
-  __syncthreads();
-  const unsigned bound = posted_bound(sh);
   for (int i = threadIdx.x; i < every; i += THREADS) {
     const Cand c = candidate(i);
-    if (score_key(c.hi) >= bound) put(c, sh);
+    top = max(top, score_key(c.hi));
+    if (every <= CAP) sh.hi[i] = c.hi, sh.lo[i] = c.lo;  // all of them have room
   }
-  const int chosen = k_highest(K, sh, bound, score_key, [&](auto see) {
+  const unsigned w = warp_mth(top, mth);
+  if (lane == 0) sh.least[warp] = w;
+  if (threadIdx.x == 0 && every <= CAP) sh.n = every;
+  __syncthreads();
+  const unsigned bound = posted_bound(sh);
+  if (every > CAP) {
+    for (int i = threadIdx.x; i < every; i += THREADS) {
+      const Cand c = candidate(i);
+      if (score_key(c.hi) >= bound) put<true>(c, sh);
+    }
+  }
+  const int chosen = k_highest<true>(K, sh, bound, score_key, [&](auto see) {
     for (int i = threadIdx.x; i < every; i += THREADS) {
       const Cand c = candidate(i);
       if (key_value64(c.hi) > -INFINITY) see(c);
