@@ -46,6 +46,34 @@ __device__ __forceinline__ float ex2(float v) {
   return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// two floats at once
+__device__ __forceinline__ u64 two(float a, float b) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void apart(u64 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // A candidate: `hi`, then `lo`, the larger one first.
 struct Cand {
   u64 hi;
@@ -60,7 +88,7 @@ struct Shared {
   unsigned lo2[CAP];
   u64 out_hi[MAX_K];
   unsigned out_lo[MAX_K];
-  unsigned least[WARPS];
+  alignas(16) unsigned least[WARPS];
   float warp_max[WARPS];
   double warp_sum[WARPS];
   double lse[MAX_W];
@@ -82,11 +110,12 @@ __device__ __forceinline__ unsigned warp_mth(unsigned top, int m) {
 }
 // The least of what the warps have posted; they post numbers that rise, so one posted before is a bound too.
 __device__ __forceinline__ unsigned posted_bound(const Shared& sh) {
-  const volatile unsigned* l = sh.least;
-  unsigned least = l[0];
-#pragma unroll
-  for (int i = 1; i < WARPS; ++i) least = min(least, (unsigned)l[i]);
-  return max(least, NOTHING + 1);
+  static_assert(WARPS == 8, "two loads of four");
+  uint32_t a, b, c, d, e, f, g, h;
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(sh.least);
+  asm volatile("ld.volatile.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(at) : "memory");
+  asm volatile("ld.volatile.shared.v4.u32 {%0, %1, %2, %3}, [%4 + 16];" : "=r"(e), "=r"(f), "=r"(g), "=r"(h) : "r"(at) : "memory");
+  return max(min(min(min(a, b), min(c, d)), min(min(e, f), min(g, h))), NOTHING + 1);
 }
 template <bool LO>
 __device__ __forceinline__ void put(const Cand& c, Shared& sh) {
@@ -177,22 +206,65 @@ __device__ __forceinline__ int place(int first, int e) { return first + (VEC ? 4
 
 template <bool VEC>
 __device__ __forceinline__ void load_batch(float (&v)[E], const float* x, int first, int V) {
-  if (VEC) {
+  if (first + BATCH <= V) {
+    if (VEC) {
 #pragma unroll
-    for (int q = 0; q < E / 4; ++q) {
-      const int i = place<VEC>(first, 4 * q);
-      if (i + 4 <= V) {
-        const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i));
+      for (int q = 0; q < E / 4; ++q) {
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(x + place<VEC>(first, 4 * q)));
         v[4 * q] = f.x, v[4 * q + 1] = f.y, v[4 * q + 2] = f.z, v[4 * q + 3] = f.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * q + e] = i + e < V ? __ldcs(x + i + e) : -INFINITY;
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = __ldcs(x + place<VEC>(first, e));
     }
-  } else {
+  } else {  // the row's last batch
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = place<VEC>(first, e) < V ? __ldcs(x + place<VEC>(first, e)) : -INFINITY;
   }
+}
+
+// What a thread knows of its part of the stretch.
+struct Walk {
+  float high = -INFINITY;  // the thread's highest logit
+  float m = -INFINITY;     // the warp's
+  float s = 0.f;           // the thread's sum of exponentials below m
+};
+
+template <bool VEC>
+__device__ __forceinline__ void walk_batch(Walk& t, const float (&v)[E], int at, bool begins, int mth, Shared& sh) {
+  constexpr float L2E = 1.4426950408889634f, L2E_LOW = (float)(1.4426950408889634 - (double)L2E);
+  float top = max3(v[0], v[1], -INFINITY);  // (a NaN is passed over here and shows in the sum)
+#pragma unroll
+  for (int e = 2; e < E; e += 2) top = max3(top, v[e], v[e + 1]);
+  t.high = fmaxf(t.high, top);
+  const unsigned key = ordered_key(t.high);
+  const float wm = key_value(__reduce_max_sync(0xffffffffu, key));
+  const unsigned w = warp_mth(key, mth);
+  if ((threadIdx.x & 31) == 0) *(volatile unsigned*)&sh.least[threadIdx.x >> 5] = w;
+  if (begins) __syncthreads();
+  const float least = key_value(posted_bound(sh));
+  if (top >= least) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (v[e] >= least) put<false>(Cand{pack(v[e], place<VEC>(at, e)), 0}, sh);
+  }
+  if (wm > t.m) {
+    t.s *= ex2((t.m - wm) * L2E);
+    t.m = wm;
+  }
+  const float below = t.m > -INFINITY ? -t.m : 0.f;
+  const u64 shift = two(below, below), scale = two(L2E, L2E), low = two(L2E_LOW, L2E_LOW);
+  u64 part = 0;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    const u64 d = add2(two(v[e], v[e + 1]), shift);  // exact for the logits that weigh most
+    float a, b;
+    apart(fma2(d, scale, mul2(d, low)), a, b);
+    part = add2(part, two(ex2(a), ex2(b)));
+  }
+  float a, b;
+  apart(part, a, b);
+  t.s += a + b;
 }
 
 // VEC: rows begin at multiples of 16 bytes, four logits a load.  All rows of a call are dealt out to threads alike, so that equal rows have
@@ -208,51 +280,25 @@ __global__ void __launch_bounds__(THREADS, 4) beam_select_kernel(BeamParams p) {
   const int first = stretch * p.batches * BATCH;
   const int batches = min(p.batches, (V - first + BATCH - 1) / BATCH);
   if (threadIdx.x == 0) sh.n = 0;
-  constexpr float L2E = 1.4426950408889634f, L2E_LOW = (float)(1.4426950408889634 - (double)L2E);
   float v[E], next[E];
-  float high = -INFINITY, m = -INFINITY, s = 0.f;  // the thread's highest logit; the warp's, and the thread's sum of exponentials below it
+  Walk t;
   pdl_wait();
   load_batch<VEC>(v, x, first, V);
-  for (int b = 0; b < batches; ++b) {
+  for (int b = 0; b < batches; b += 2) {
     const int at = first + b * BATCH;
     if (b + 1 < batches) load_batch<VEC>(next, x, at + BATCH, V);
-    float top = v[0];
-#pragma unroll
-    for (int e = 1; e < E; ++e) top = fmaxf(top, v[e]);  // (a NaN is passed over here and shows in the sum)
-    top = fmaxf(top, -INFINITY);
-    high = fmaxf(high, top);
-    const unsigned key = ordered_key(high);
-    const float wm = key_value(__reduce_max_sync(0xffffffffu, key));
-    const unsigned w = warp_mth(key, mth);
-    if (lane == 0) *(volatile unsigned*)&sh.least[warp] = w;
-    if (b == 0) __syncthreads();
-    const float least = key_value(posted_bound(sh));
-    if (top >= least) {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (v[e] >= least) put<false>(Cand{pack(v[e], place<VEC>(at, e)), 0}, sh);
+    walk_batch<VEC>(t, v, at, b == 0, mth, sh);
+    if (b + 1 < batches) {
+      if (b + 2 < batches) load_batch<VEC>(v, x, at + 2 * BATCH, V);
+      walk_batch<VEC>(t, next, at + BATCH, false, mth, sh);
     }
-    if (wm > m) {
-      s *= ex2((m - wm) * L2E);
-      m = wm;
-    }
-    const float below = m > -INFINITY ? m : 0.f;
-    float part = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float d = v[e] - below;  // exact for the logits that weigh most
-      part += ex2(fmaf(d, L2E, d * L2E_LOW));
-    }
-    s += part;
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = next[e];
   }
   {
-    double d = s;
+    double d = t.s;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
     if (lane == 0) {
-      sh.warp_max[warp] = m;
+      sh.warp_max[warp] = t.m;
       sh.warp_sum[warp] = d;
     }
   }
@@ -284,9 +330,9 @@ __global__ void __launch_bounds__(THREADS, 4) beam_select_kernel(BeamParams p) {
   __syncthreads();
   if (threadIdx.x == 0) {
     // what the CTA wrote is seen by whoever sees its ticket
-    int t;
-    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(t) : "l"(p.tickets + prompt) : "memory");
-    sh.last = t == p.W * p.stretches - 1;
+    int done;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(done) : "l"(p.tickets + prompt) : "memory");
+    sh.last = done == p.W * p.stretches - 1;
     if (sh.last) p.tickets[prompt] = 0;
     sh.n = 0;
   }
@@ -325,8 +371,11 @@ __global__ void __launch_bounds__(THREADS, 4) beam_select_kernel(BeamParams p) {
     return Cand{ordered_key64(sc), 0xffffffffu - ((unsigned)b * V + (0xffffffffu - (unsigned)c))};
   };
   auto score_key = [](u64 hi) { return ordered_key((float)key_value64(hi)); };
+  // (a stretch's candidates are in order: every warp takes some of all ranks, or the least of the warps' bounds would be a low one)
   unsigned top = 0;
-  for (int i = threadIdx.x; i < every; i += THREADS) {
+  for (int i0 = 0, turn = 0; i0 < every; i0 += THREADS, turn += 37) {
+    const int i = i0 + ((threadIdx.x * 5 + turn) & (THREADS - 1));
+    if (i >= every) continue;
     const Cand c = candidate(i);
     top = max(top, score_key(c.hi));
     if (every <= CAP) sh.hi[i] = c.hi, sh.lo[i] = c.lo;  // all of them have room
