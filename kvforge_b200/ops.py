@@ -99,7 +99,8 @@ _SIGNATURES = {
     "kvf_copy_states": "pilppiiip",
     "kvf_beams_set_pdl": "i",
     # library "adapters"
-    "kvf_adapter_add_{s}": "plppppp" + "i" * 6 + "i" * 4 + "plplipp",
+    "kvf_adapter_add_{s}": "plppppp" + "i" * 6 + "i" * 4 + "plplippipp",
+    "kvf_adapter_group": "piiiipppp",
     "kvf_adapters_set_pdl": "i",
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
@@ -2880,17 +2881,27 @@ class AdapterBank:
         self.size, self.sections, self.rank, self.k, self.n = s, sections, r, k, n
 
 
+ADAPTER_DIRECT = 64  # up to so many rows the kernels group for themselves
+ADAPTER_TILE = 16  # rows of one adapter that a tile has room for
+
+
 class AdapterGroups:
-    """Which rows of a step take which adapter: made once for up to ``max_tokens`` rows and ``num_adapters`` adapters, filled by
-    ``group_by_adapter`` and read by every ``adapter_add`` of the step."""
+    """Which rows of a step take which adapter: made once for up to ``max_tokens`` rows and a bank's ``num_adapters`` adapters, filled by
+    ``group_by_adapter`` and read by every ``adapter_add`` of the step.  One step at a time uses it."""
 
     def __init__(self, max_tokens: int, num_adapters: int, device: torch.device | str) -> None:
-        if max_tokens < 1 or num_adapters < 1:
-            raise ValueError("groups of adapters need room for a row and an adapter")
+        if max_tokens < 1 or not 1 <= num_adapters <= 4096:
+            raise ValueError("groups of adapters need room for a row and 1 to 4,096 adapters")
         self.max_tokens, self.num_adapters = int(max_tokens), int(num_adapters)
-        self.device = torch.device(device)
+        self.rows = torch.empty(self.max_tokens, dtype=torch.int32, device=device)
+        self.tiles = torch.empty(3 * self.max_tiles(self.max_tokens), dtype=torch.int32, device=device)
         self.ids: torch.Tensor | None = None
+        self.err: torch.Tensor | None = None
         self.n = 0
+
+    def max_tiles(self, n: int) -> int:
+        """The most tiles that ``n`` rows can make (rows without an adapter make tiles too)."""
+        return n // ADAPTER_TILE + min(self.num_adapters + 1, n)
 
 
 def group_by_adapter(ids: torch.Tensor, groups: AdapterGroups, err: torch.Tensor | None = None) -> None:
@@ -2898,10 +2909,14 @@ def group_by_adapter(ids: torch.Tensor, groups: AdapterGroups, err: torch.Tensor
     the step's last ``adapter_add``.  An id outside the bank counts as -1 and sets bit 32 of ``err``."""
     if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous():
         raise ValueError("group_by_adapter: ids are contiguous int32, one a row")
-    if ids.numel() > groups.max_tokens:
-        raise ValueError(f"group_by_adapter: {ids.numel()} rows, but the groups were made for {groups.max_tokens}")
-    _here(ids, err)
-    groups.ids, groups.n, groups.err = ids, ids.numel(), err
+    n = ids.numel()
+    if n > groups.max_tokens:
+        raise ValueError(f"group_by_adapter: {n} rows, but the groups were made for {groups.max_tokens}")
+    _here(ids, groups.rows, err)
+    groups.ids, groups.n, groups.err = ids, n, err
+    if n > ADAPTER_DIRECT:
+        name = "kvf_adapter_group"
+        _check(_fn(name, "adapters")(_ptr(ids), n, groups.num_adapters, ADAPTER_TILE, groups.max_tiles(n), _ptr(groups.rows), _ptr(groups.tiles), _ptr(err), _stream()), name)
 
 
 def adapter_add(x: torch.Tensor, bank: AdapterBank, groups: AdapterGroups, out: torch.Tensor, base: torch.Tensor | None = None) -> None:
@@ -2911,7 +2926,7 @@ def adapter_add(x: torch.Tensor, bank: AdapterBank, groups: AdapterGroups, out: 
     n, k = x.shape
     if x.dtype != bank.a.dtype or k != bank.k or x.stride(1) != 1 or (x.stride(0) * x.element_size()) % 16 or x.data_ptr() % 16:
         raise ValueError("adapter_add: x must be [N, K] of the bank's type and width, its rows at multiples of 16 bytes")
-    if groups.n != n or groups.ids is None or groups.num_adapters < bank.size:
+    if groups.n != n or groups.ids is None or groups.num_adapters != bank.size:
         raise ValueError("adapter_add: the groups are not those of these rows and this bank")
     base = out if base is None else base
     for t, what in ((out, "out"), (base, "base")):
@@ -2925,11 +2940,13 @@ def adapter_add(x: torch.Tensor, bank: AdapterBank, groups: AdapterGroups, out: 
     if n == 0:
         return
     ends = (*bank.ends, bank.n, bank.n)
+    listed = n > ADAPTER_DIRECT
     name = f"kvf_adapter_add_{s}"
     _check(
         _fn(name, "adapters")(
             _ptr(x), x.stride(0), _ptr(bank.a), _ptr(bank.b), _ptr(bank.scales), _ptr(bank.ranks), _ptr(groups.ids), n, bank.size, bank.sections, bank.rank, k, bank.n,
-            ends[0], ends[1], ends[2], int(bank.alternating), _ptr(base), base.stride(0), _ptr(out), out.stride(0), int(out.dtype == torch.float32), _ptr(groups.err), _stream(),
+            ends[0], ends[1], ends[2], int(bank.alternating), _ptr(base), base.stride(0), _ptr(out), out.stride(0), int(out.dtype == torch.float32),
+            _ptr(groups.rows), _ptr(groups.tiles) if listed else None, groups.max_tiles(n) if listed else 0, _ptr(groups.err), _stream(),
         ),
         name,
     )  # fmt: skip
