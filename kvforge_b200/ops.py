@@ -99,7 +99,7 @@ _SIGNATURES = {
     "kvf_copy_states": "pilppiiip",
     "kvf_beams_set_pdl": "i",
     # library "adapters"
-    "kvf_adapter_add_{s}": "plppppp" + "i" * 6 + "i" * 4 + "plplippipp",
+    "kvf_adapter_add_{s}": "plppppp" + "i" * 6 + "i" * 4 + "plplippipipp",
     "kvf_adapter_group": "piiiipppp",
     "kvf_adapters_set_pdl": "i",
 }
@@ -2882,19 +2882,25 @@ class AdapterBank:
 
 
 ADAPTER_DIRECT = 64  # up to so many rows the kernels group for themselves
-ADAPTER_TILE = 16  # rows of one adapter that a tile has room for
+ADAPTER_MANY = 256  # from so many bfloat16 rows on the two products are kernels of their own
+ADAPTER_TILE = 64  # rows of one adapter that a tile of the list has room for
 
 
 class AdapterGroups:
     """Which rows of a step take which adapter: made once for up to ``max_tokens`` rows and a bank's ``num_adapters`` adapters, filled by
-    ``group_by_adapter`` and read by every ``adapter_add`` of the step.  One step at a time uses it."""
+    ``group_by_adapter`` and read by every ``adapter_add`` of the step.  One step at a time uses it.  ``max_rows``: rows of ``a`` (ranks times
+    sections) of the largest bank it is used with."""
 
-    def __init__(self, max_tokens: int, num_adapters: int, device: torch.device | str) -> None:
-        if max_tokens < 1 or not 1 <= num_adapters <= 4096:
-            raise ValueError("groups of adapters need room for a row and 1 to 4,096 adapters")
+    def __init__(self, max_tokens: int, num_adapters: int, device: torch.device | str, max_rows: int = ADAPTER_MAX_ROWS) -> None:
+        if max_tokens < 1 or not 1 <= num_adapters <= 4096 or not 16 <= max_rows <= ADAPTER_MAX_ROWS:
+            raise ValueError("groups of adapters need room for a row, 1 to 4,096 adapters and ranks of 16 or more")
         self.max_tokens, self.num_adapters = int(max_tokens), int(num_adapters)
         self.rows = torch.empty(self.max_tokens, dtype=torch.int32, device=device)
         self.tiles = torch.empty(3 * self.max_tiles(self.max_tokens), dtype=torch.int32, device=device)
+        # what lies between the two products of many rows: three 16-bit numbers each at most
+        wide = self.max_tiles(self.max_tokens) * ADAPTER_TILE * 3 * max_rows if self.max_tokens >= ADAPTER_MANY else 0
+        self.inner = torch.empty(wide, dtype=torch.bfloat16, device=device)
+        self.max_rows = int(max_rows)
         self.ids: torch.Tensor | None = None
         self.err: torch.Tensor | None = None
         self.n = 0
@@ -2939,6 +2945,9 @@ def adapter_add(x: torch.Tensor, bank: AdapterBank, groups: AdapterGroups, out: 
     _here(x, bank.a, out, base, groups.ids)
     if n == 0:
         return
+    if bank.sections * bank.rank > groups.max_rows:
+        raise ValueError(f"adapter_add: the groups were made for {groups.max_rows} rows of a bank's adapters, this bank's have {bank.sections * bank.rank}")
+    two = n >= ADAPTER_MANY and s == "bf16"
     ends = (*bank.ends, bank.n, bank.n)
     listed = n > ADAPTER_DIRECT
     name = f"kvf_adapter_add_{s}"
@@ -2946,7 +2955,8 @@ def adapter_add(x: torch.Tensor, bank: AdapterBank, groups: AdapterGroups, out: 
         _fn(name, "adapters")(
             _ptr(x), x.stride(0), _ptr(bank.a), _ptr(bank.b), _ptr(bank.scales), _ptr(bank.ranks), _ptr(groups.ids), n, bank.size, bank.sections, bank.rank, k, bank.n,
             ends[0], ends[1], ends[2], int(bank.alternating), _ptr(base), base.stride(0), _ptr(out), out.stride(0), int(out.dtype == torch.float32),
-            _ptr(groups.rows), _ptr(groups.tiles) if listed else None, groups.max_tiles(n) if listed else 0, _ptr(groups.err), _stream(),
+            _ptr(groups.rows), _ptr(groups.tiles) if listed else None, groups.max_tiles(n) if listed else 0, _ptr(groups.inner) if two else None,
+            int(two), _ptr(groups.err), _stream(),
         ),
-        name,
+        name, 2 if two else 1,
     )  # fmt: skip
