@@ -3,20 +3,21 @@
 // and base[n] where s is -1.  A section is one of the matrices that are stacked in the projection (queries, keys, values);
 // of gates and ups that alternate in blocks of 8 columns the sections alternate too.
 //
-// Neither product needs its operands in shared memory: a lane takes 16 bytes of a row at a time, and which of its k come first in a
-// tensor-core step is its own affair as long as x and A (or the inner numbers and B) agree.  bfloat16 goes to the tensor cores
-// (mma.sync m16n8k16: sixteen flops or so a byte of x and of A, so bytes and latency bound it, not the products); the numbers between the two
-// products are sums in 32 bits and are multiplied as two bfloat16 numbers (2^-17 of each is lost beside a result that is rounded to
-// 2^-8), or as three where the result is float.  float32 stays on the FP32 pipes.
+// bfloat16, the first product: on the tcgen05 tensor cores, by a cluster of eight CTAs that share out k in blocks of 64 columns; the adapter's
+// rows of A are the 128 lanes of the accumulator, the tile's rows its columns, so that 16 rows cost as little as a product of 128 x 16 and no
+// register holds what is on its way (A comes by TMA, the rows of x gathered by TMA four at a time, several blocks ahead).  Rows of A past the
+// adapter's are whatever lies there in shared memory: their lanes are not read.  Every CTA's sums go to the CTAs that need them through shared memory and are added in
+// one order.
+// The second product has 16 to 128 k and thousands of columns, each read and written once: mma.sync with operands straight from
+// memory (a lane takes eight bytes of a row of B; which of its k come first is its own affair as long as the inner numbers agree), bound
+// by the rows that are read and written.  The numbers between the products are sums in 32 bits and are multiplied as two bfloat16 numbers
+// (2^-17 of each is lost beside a result that is rounded to 2^-8), or as three where the result is float.  float32 stays on the FP32 pipes.
 //
-// Few rows (and float32): one launch.  16 rows of one adapter go to a cluster of eight CTAs: their 64 warps share out the columns of x and A,
-// the partial sums meet in shared memory (of the CTA, then of every CTA of the cluster, summed in one order), and each CTA adds its
-// eighth of the result's columns.
-// Many rows: two launches.  64 rows of one adapter go to a cluster of eight CTAs that make their inner numbers, and then to a CTA every 256
-// columns of the result: the first kernel reads x once, the second reads and writes the rows once.
+// Few rows (and float32): one launch, a cluster makes 16 rows' inner numbers in all its CTAs and then each CTA an eighth of the columns.
+// Many rows: two launches.  A cluster makes 128 rows' inner numbers; then 64 rows and some hundred columns are a CTA.
 //
 // Which rows make a tile: up to 64 rows every cluster finds out for itself; for more a kernel of one CTA sorts the rows once a step.
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 using namespace kvf;
 
@@ -26,13 +27,13 @@ constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_SECTIONS = 4;
 constexpr int TILE = 16;        // rows of a cluster that makes both products
-constexpr int LIST = 64;        // rows of a tile of the list
+constexpr int LIST = 128;       // rows of a tile of the list
 constexpr int CLUSTER = 8;      // CTAs a tile
 constexpr int DIRECT = 64;      // up to so many rows are grouped by every cluster itself
 constexpr int CHUNK = 48;       // rows of A a warp multiplies at a time
 constexpr int PART = CHUNK + 4; // floats from one row of the partial sums to the next
 constexpr int AHEAD = 2;        // groups of columns that a warp fetches ahead
-constexpr int MOST = 256;       // numbers between the products of a row that are in shared memory at a time (whole sections)
+constexpr int MOST = 192;       // numbers between the products of a row that are in shared memory at a time (whole sections)
 
 struct AdapterParams {
   const void* x;
@@ -52,6 +53,9 @@ struct AdapterParams {
   // sections: where they begin, how wide they are, and the groups of 32 columns up to their end
   int begin[MAX_SECTIONS], width[MAX_SECTIONS], groups[MAX_SECTIONS];
   int alternating;
+  int most;   // inner numbers of a row that shared memory holds at a time (whole sections of rank R)
+  int slots;  // blocks of 64 columns of k that it holds (bf16)
+  int tmem;   // columns of tensor memory
 };
 
 // A section as a lane needs it (taken from the parameters with fixed indices: an index known only at run time costs a constant load's
@@ -83,61 +87,32 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t cta, float4 v
       "st.shared::cluster.v4.f32 [at], {%2, %3, %4, %5};\n\t}" ::"r"(addr), "r"(cta), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                 "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(at)
+               : "memory");
+}
+// (naming the registers keeps the compiler from using them before the wait)
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // Column of the result that is number u of a section.
 __device__ __forceinline__ int column(const AdapterParams& p, const Section& s, int u) { return p.alternating ? (u >> 3) * 16 + s.sec * 8 + (u & 7) : s.begin + u; }
 
-// ---- the first product: partial sums over a warp's share of k for 16 rows and CHUNK rows of A, into part[16][PART]
+// ---- the first product in float32: partial sums over a warp's share of k for 16 rows and CHUNK rows of A, into part[16][PART]
 // k goes in steps of 32, eight a lane; step st belongs to warp st % 64 of the cluster
 struct Rows {
   const char* lo;  // the lane's row g, or null
   const char* hi;  // and g + 8
 };
-
-__device__ __forceinline__ void first_product(const AdapterParams& p, const bf16* a, const Rows& x, int t0, int total, int R16, int gw, float* part) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  float acc[CHUNK / 8][4];
-#pragma unroll
-  for (int j = 0; j < CHUNK / 8; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
-  const bf16* rows[CHUNK / 8];
-#pragma unroll
-  for (int j = 0; j < CHUNK / 8; ++j) {
-    const int t = t0 + j * 8 + g;
-    const int sec = (t >= R16) + (t >= 2 * R16) + (t >= 3 * R16);
-    rows[j] = t < total ? a + (long long)(sec * (p.R - R16) + t) * p.K : nullptr;
-  }
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  constexpr int STEP = 32 * CLUSTER * WARPS;
-  for (int k0 = gw * 32; k0 < p.K; k0 += 2 * STEP) {  // (all lanes take every step: K may end inside one)
-    // the loads of two steps go out together
-    uint4 lo[2], hi[2], w[2][CHUNK / 8];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int k = k0 + i * STEP + q * 8;
-      const bool in = k < p.K;
-      lo[i] = x.lo && in ? __ldg(reinterpret_cast<const uint4*>(x.lo + 2ll * k)) : zero;
-      hi[i] = x.hi && in ? __ldg(reinterpret_cast<const uint4*>(x.hi + 2ll * k)) : zero;
-#pragma unroll
-      for (int j = 0; j < CHUNK / 8; ++j) w[i][j] = rows[j] && in ? __ldg(reinterpret_cast<const uint4*>(rows[j] + k)) : zero;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int j = 0; j < CHUNK / 8; ++j) {
-        mma(acc[j], lo[i].x, hi[i].x, lo[i].y, hi[i].y, w[i][j].x, w[i][j].y);
-        mma(acc[j], lo[i].z, hi[i].z, lo[i].w, hi[i].w, w[i][j].z, w[i][j].w);
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < CHUNK / 8; ++j) {
-    *reinterpret_cast<float2*>(part + g * PART + j * 8 + 2 * q) = make_float2(acc[j][0], acc[j][1]);
-    *reinterpret_cast<float2*>(part + (g + 8) * PART + j * 8 + 2 * q) = make_float2(acc[j][2], acc[j][3]);
-  }
-}
 
 __device__ __forceinline__ float dot8(const float4& a0, const float4& a1, const float4& b0, const float4& b1, float c) {
   c = fmaf(a0.x, b0.x, c), c = fmaf(a0.y, b0.y, c), c = fmaf(a0.z, b0.z, c), c = fmaf(a0.w, b0.w, c);
@@ -181,6 +156,146 @@ __device__ __forceinline__ void first_product(const AdapterParams& p, const floa
   }
 }
 
+// ---- the first product in bfloat16
+constexpr int BLOCK_K = 64;  // columns of a block: a 128-byte row of the swizzled tiles
+constexpr int MAX_SLOTS = WARPS - 1;  // (a slot has a warp of its own that fills it)
+constexpr int BARS = 2 * MAX_SLOTS + 1;
+constexpr int SUM_ROW = 20;  // floats from the sums of one row of A to the next's: of 16 rows of x, and room against bank conflicts
+
+struct Maps {
+  CUtensorMap x, run, a;  // rows of x, twice, and of all adapters' A, 64 columns a box: one row, 32 rows, sixteen rows
+};
+
+struct Tensor {
+  uint32_t ring, bars, tmem;  // blocks ([NR rows of x | rows of A] each); barriers: a slot is filled, its products are done, all are; accumulator
+  int block, pass;            // blocks and passes so far: what phase the barriers are in
+};
+
+__host__ __device__ constexpr int slot_bytes(int nr, int rows) { return (nr + rows) * BLOCK_K * 2; }
+
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, int y0, int y1, int y2, int y3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y0), "r"(y1), "r"(y2), "r"(y3), "r"(bar)
+      : "memory");
+}
+
+// This CTA's share of a[total rows][k] x[NR rows][k], sent to where it is needed: the sums of `sums[rank][t][SUM_ROW]`, of all 16 rows in every CTA of
+// the cluster (NR = 16), or of rows 16c .. 16c + 15 in CTA c (NR = 128).  a0: the first of the sections' rows of A among all adapters'; rows:
+// of x, each valid; runs: bit i, rows 32i .. 32i + 31 follow one another in x.  Blocks are the cluster's in turn: block j of the CTA is block
+// rank + 8 j of k.  Warp 0 multiplies; a block is fetched by one thread of another warp (a warp takes some 90 cycles for each copy that it
+// starts: all of eight blocks by one warp kept eight rows and 4096 columns waiting for 5,700 cycles).
+template <int NR>
+__device__ __forceinline__ void first_product(const AdapterParams& p, const Maps& maps, int a0, const int* rows, unsigned runs, int total, int R16, int rank, Tensor& tn, float* sums) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int every = (p.K + BLOCK_K - 1) / BLOCK_K, blocks = (every - rank + CLUSTER - 1) / CLUSTER;  // (none for some where K is short)
+  const uint32_t bytes = slot_bytes(NR, total), filled = tn.bars, done = filled + 8 * MAX_SLOTS, all = done + 8 * MAX_SLOTS;
+  const int tiles = (total + 127) / 128;
+  if (warp > 0) {
+    // Warp w fills slot w - 1 and no other, one block after another: what it waits for is never more than one phase ahead of the barrier
+    // (a parity tells only two neighbouring phases apart).
+    if (warp <= p.slots && elect_one()) {
+      const int slot = warp - 1, begin = tn.block % p.slots;
+      for (int j = slot - begin + (slot < begin ? p.slots : 0); j < blocks; j += p.slots) {
+        const int turn = (tn.block + j) / p.slots;
+        if (turn) tc::bar_wait(done + 8 * slot, (turn - 1) & 1, p.err);
+        const uint32_t to = tn.ring + slot * bytes, bar = filled + 8 * slot;
+        tc::bar_expect_tx(bar, bytes);
+        const int k = (rank + CLUSTER * j) * BLOCK_K;
+        for (int t = 0, sec = 0, in = 0; t < total; t += 16) {
+          tc::tma_load_2d(to + (NR + t) * 128, &maps.a, k, a0 + sec * p.R + in, bar);
+          in += 16;
+          if (in == R16) in = 0, ++sec;
+        }
+#pragma unroll
+        for (int i = 0; i < (NR + 31) / 32; ++i) {
+          if (runs >> i & 1) {
+            tc::tma_load_2d(to + i * 4096, &maps.run, k, rows[32 * i], bar);
+          } else {
+#pragma unroll
+            for (int r = 32 * i; r < min(NR, 32 * i + 32); r += 4) tma_gather4(to + r * 128, &maps.x, k, rows[r], rows[r + 1], rows[r + 2], rows[r + 3], bar);
+          }
+        }
+      }
+    }
+  } else {
+    int slot = tn.block % p.slots, turn = tn.block / p.slots;
+    for (int j = 0; j < blocks; ++j) {
+      tc::bar_wait(filled + 8 * slot, turn & 1, p.err);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (elect_one()) {
+        const uint32_t at = tn.ring + slot * bytes;
+        for (int m = 0; m < tiles; ++m) {
+          const uint64_t da = tc::sdesc(at + NR * 128 + m * 128 * 128), db = tc::sdesc(at);
+#pragma unroll
+          for (int i = 0; i < BLOCK_K / 16; ++i) tc::umma(tn.tmem + m * NR, da + 2 * i, db + 2 * i, tc::idesc(NR, 0), j | i);
+        }
+        tc::umma_commit(done + 8 * slot);
+        if (j + 1 == blocks) tc::umma_commit(all);
+      }
+      __syncwarp();
+      if (++slot == p.slots) slot = 0, ++turn;
+    }
+  }
+  __syncwarp();
+  if (blocks > 0) {
+    tc::bar_wait(all, tn.pass & 1, p.err);
+    tn.block += blocks;
+    ++tn.pass;
+  }
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  // the CTAs of the cluster run, and have read the sums of the sections before: their memory may be written
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  // warps w and w + 4 have the same lanes of the accumulator: the first goes to CTAs 0 .. 3, the second to 4 .. 7
+  for (int m = 0; m < tiles; ++m) {
+    const int t = m * 128 + (warp & 3) * 32;
+    if (t >= total) break;
+    const uint32_t from = tn.tmem + m * NR + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t to = sm32(sums + (rank * total + t + lane) * SUM_ROW);
+    uint32_t r[16];
+    if (NR == 16) {
+      tmem_ld16(from, r);
+      tmem_wait16(r);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int cta = (warp >> 2) * 4 + i;
+      if (NR != 16) {
+        tmem_ld16(from + cta * 16, r);
+        tmem_wait16(r);
+      }
+      if (t + lane < total) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4 v = blocks > 0 ? make_float4(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1]), __uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3]))
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+          st_cluster(to + 16 * e, cta, v);
+        }
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+
+// Barriers and tensor memory of a CTA (by all threads; ends with a barrier); what the CTA's ring begins with lies at a multiple of 1,024 bytes.
+__device__ __forceinline__ Tensor make_tensor(const AdapterParams& p, float* ring, unsigned long long* bars, uint32_t* slot) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < BARS; ++i) tc::bar_init(sm32(bars + i), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x < 32) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm32(slot)), "r"(p.tmem) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  return Tensor{sm32(ring), sm32(bars), *slot, 0, 0};
+}
+__device__ __forceinline__ void free_tensor(const AdapterParams& p, const Tensor& tn) {
+  if (threadIdx.x < 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tn.tmem), "r"(p.tmem) : "memory");
+}
+
 // ---- the numbers between the products in shared memory, and the second product: 16 rows and 32 columns a warp
 // (bf16: `SPLITS` numbers of 16 bits that add up to each; a row's stride makes the eight rows of a load lie in different banks)
 __host__ __device__ inline int inner_stride(int total, int size) { return size == 4 ? total + 4 : total % 32 == 0 ? total + 16 : total; }
@@ -205,15 +320,15 @@ __device__ __forceinline__ void keep_inner(float* inner, int total, int row, int
 // sixteen numbers of its rows of B (bf16) and the rows that are added to.
 template <typename T, typename O>
 struct Group {
-  Section s;         // sec < 0: none
-  int u0;            // its first column in the section
-  int col;           // the lane's first column of the result, or -1
-  uint2 w[4];        // bf16: B
+  int gi;        // its number, or -1
+  int col;       // the lane's first column of the result, or -1
+  uint2 w[4];    // bf16: B
   uint4 base[2][sizeof(O) / 2];
 };
 
+// Row of B for the lane's column of the j-th of four tensor-core tiles: column 2q + e of it is column 8q + 2j + e of the 32, so that a lane's
+// eight results lie side by side.
 __device__ __forceinline__ const bf16* b_row(const AdapterParams& p, const bf16* b, const Section& s, int u0, int j) {
-  // column 2q + e of the j-th of four tensor-core tiles is column 8q + 2j + e of the 32: a lane's eight results lie side by side
   const int g = (threadIdx.x & 31) >> 2, u = u0 + (g >> 1) * 8 + 2 * j + (g & 1);
   return u < s.width ? b + (long long)column(p, s, u) * p.R : nullptr;
 }
@@ -222,13 +337,15 @@ template <typename T, typename O>
 __device__ __forceinline__ void fetch(Group<T, O>& gr, const AdapterParams& p, const T* b, const O* base0, const O* base1) {
   const int q = threadIdx.x & 3;
   gr.col = -1;
-  if (gr.s.sec < 0) return;
-  const int u = gr.u0 + 8 * q;
-  if (u < gr.s.width) gr.col = column(p, gr.s, u);
+  if (gr.gi < 0) return;
+  int gi = gr.gi;
+  const Section s = section_of_group(p, gi);
+  const int u = gi * 32 + 8 * q;
+  if (u < s.width) gr.col = column(p, s, u);
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const T* row = b_row(p, b, gr.s, gr.u0, j);
+      const T* row = b_row(p, b, s, gi * 32, j);
       gr.w[j] = row ? __ldg(reinterpret_cast<const uint2*>(row + 4 * q)) : make_uint2(0, 0);
     }
   }
@@ -239,30 +356,32 @@ __device__ __forceinline__ void fetch(Group<T, O>& gr, const AdapterParams& p, c
   }
 }
 
-// acc[row half][column]: eight columns a lane
+// acc[row half][column]: eight columns a lane; sec0: the section that `inner` begins with
 template <int SPLITS, typename O>
-__device__ __forceinline__ void second_product(const AdapterParams& p, const bf16* b, const bf16* inner, int total, const Group<bf16, O>& gr, int R16, float (&acc)[2][8]) {
+__device__ __forceinline__ void second_product(const AdapterParams& p, const bf16* b, const bf16* inner, int total, int sec0, const Group<bf16, O>& gr, int R16, float (&acc)[2][8]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int stride = inner_stride(total, 2);
+  int gi = gr.gi;
+  const Section s = section_of_group(p, gi);
   float c[4][4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
+  const bf16* mine = inner + g * stride + (s.sec - sec0) * R16 + 4 * q;
   for (int r0 = 0; r0 < R16; r0 += 16) {
     uint2 w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (r0 == 0) {
-        w[j] = gr.w[j];
-      } else {
-        const bf16* row = b_row(p, b, gr.s, gr.u0, j);
+      w[j] = gr.w[j];
+      if (r0) {
+        const bf16* row = b_row(p, b, s, gi * 32, j);
         w[j] = row ? __ldg(reinterpret_cast<const uint2*>(row + r0 + 4 * q)) : make_uint2(0, 0);
       }
     }
 #pragma unroll
     for (int i = 0; i < SPLITS; ++i) {
-      const bf16* h = inner + (i * TILE + g) * stride + r0 + 4 * q;
+      const bf16* h = mine + i * TILE * stride + r0;
       const uint2 lo = *reinterpret_cast<const uint2*>(h), hi = *reinterpret_cast<const uint2*>(h + 8 * stride);
 #pragma unroll
       for (int j = 0; j < 4; ++j) mma(c[j], lo.x, hi.x, lo.y, hi.y, w[j].x, w[j].y);
@@ -276,14 +395,16 @@ __device__ __forceinline__ void second_product(const AdapterParams& p, const bf1
 }
 
 template <int SPLITS, typename O>
-__device__ __forceinline__ void second_product(const AdapterParams& p, const float* b, const float* inner, int total, const Group<float, O>& gr, int R16, float (&acc)[2][8]) {
+__device__ __forceinline__ void second_product(const AdapterParams& p, const float* b, const float* inner, int total, int sec0, const Group<float, O>& gr, int R16, float (&acc)[2][8]) {
   const int lane = threadIdx.x & 31, g = lane >> 2;
   const int stride = inner_stride(total, 4);
+  int gi = gr.gi;
+  const Section s = section_of_group(p, gi);
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[0][i] = acc[1][i] = 0.f;
   if (gr.col < 0) return;
   const float* rows = b + (long long)gr.col * p.R;
-  const float* lo = inner + g * stride;
+  const float* lo = inner + g * stride + (s.sec - sec0) * R16;
   const float* hi = lo + 8 * stride;
   for (int r = 0; r < R16; r += 4) {
     const float4 l = *reinterpret_cast<const float4*>(lo + r), h = *reinterpret_cast<const float4*>(hi + r);
@@ -363,12 +484,16 @@ __device__ __forceinline__ int own_rows(const AdapterParams& p, int t, int* rows
 
 // T: type of x, A and B; O: of base and out
 template <typename T, typename O, int SPLITS>
-__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) adapter_tile_kernel(const __grid_constant__ AdapterParams p) {
-  extern __shared__ __align__(16) float smem[];  // the warps' partial sums (then the numbers between the products), the CTAs' sums
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) adapter_tile_kernel(const __grid_constant__ AdapterParams p, const __grid_constant__ Maps maps) {
+  // float32: the warps' partial sums (whose place the inner numbers take), then the CTAs' sums.  bfloat16: the ring of blocks, the sums, the inner numbers.
+  extern __shared__ __align__(1024) float smem[];
   __shared__ int rows[TILE];
-  pdl_launch();
+  __shared__ __align__(8) unsigned long long bars[BARS];
+  __shared__ uint32_t tmem_slot;
+  constexpr bool TENSOR = sizeof(T) == 2;
+  if (!TENSOR) pdl_launch();
   pdl_wait();
-  const int tile = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;  // (of the list: a quarter of a tile)
+  const int tile = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;  // (of the list: part of a tile)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
   int s, count;
   if (p.tiles) {
@@ -380,9 +505,9 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
     count = own_rows(p, tile, rows, s);
   }
   if (count <= 0) return;  // (the whole cluster)
-  __syncthreads();
   const int R = s < 0 ? 0 : p.ranks ? min(max(p.ranks[s], 0), p.R) : p.R;
   if (R == 0) {
+    __syncthreads();
     copy_rows<O>(p, rows, count, rank, CLUSTER);
     return;
   }
@@ -390,6 +515,15 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
   const int R16 = (R + 15) & ~15;
   const T* a = reinterpret_cast<const T*>(p.a) + (long long)s * p.sections * p.R * p.K;
   const T* b = reinterpret_cast<const T*>(p.b) + (long long)s * p.N * p.R;
+  // whole sections at a time, as many as there is room for
+  const int together = min(p.sections, p.most / R16);
+  Tensor tn;
+  if constexpr (TENSOR) {
+    tn = make_tensor(p, smem, bars, &tmem_slot);  // (a barrier: the rows are there)
+    pdl_launch();                                 // not before it has its tensor memory: a kernel that waits for this one could hold it
+    if (threadIdx.x >= count && threadIdx.x < TILE) rows[threadIdx.x] = rows[0];  // (any row: what comes of it is not read)
+  }
+  __syncthreads();
   // this CTA's eighth of B and of the rows that are added to comes on its way
   const int per = (p.N / 8 + CLUSTER - 1) / CLUSTER * 8, c0 = rank * per, c1 = min(p.N, c0 + per);
   if (c0 < c1) {
@@ -402,14 +536,11 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
       for (int i = threadIdx.x % (THREADS / TILE) * 128; i < row_bytes; i += 128 * (THREADS / TILE)) prefetch(at + i);
     }
   }
-
-  // whole sections at a time, as many as there is room for
-  const int together = min(p.sections, MOST / R16);
-  float* part = smem;                        // [WARPS][TILE][PART]
-  float* sums = part + WARPS * TILE * PART;  // [CLUSTER][TILE][total]
-  T* inner = reinterpret_cast<T*>(part);     // (once the partial sums are out of the way)
+  float* part = smem;                       // float32: [WARPS][TILE][PART]
+  float* sums = TENSOR ? reinterpret_cast<float*>(reinterpret_cast<char*>(smem) + p.slots * slot_bytes(TILE, p.most)) : smem + WARPS * TILE * PART;
+  T* inner = TENSOR ? reinterpret_cast<T*>(sums + CLUSTER * p.most * SUM_ROW) : reinterpret_cast<T*>(smem);
   Rows x;
-  {
+  if constexpr (!TENSOR) {
     const char* from = reinterpret_cast<const char*>(p.x);
     x.lo = g < count ? from + rows[g] * p.x_stride * (long long)sizeof(T) : nullptr;
     x.hi = g + 8 < count ? from + rows[g + 8] * p.x_stride * (long long)sizeof(T) : nullptr;
@@ -421,324 +552,332 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
   O* out1 = g + 8 < count ? reinterpret_cast<O*>(p.out) + rows[g + 8] * p.out_stride : nullptr;
   for (int sec0 = 0; sec0 < p.sections; sec0 += together) {
     const int sec1 = min(p.sections, sec0 + together), total = (sec1 - sec0) * R16;
-    for (int t0 = 0; t0 < total; t0 += CHUNK) {
-      first_product(p, a + (long long)sec0 * p.R * p.K, x, t0, total, R16, rank * WARPS + warp, part + warp * TILE * PART);
-      // the CTAs of the cluster run, and have read the sums of the sections before: their memory may be written
-      if (t0 == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-      __syncthreads();
-      const int wide = min(CHUNK, total - t0);
-      const int row = threadIdx.x / (THREADS / TILE), t = threadIdx.x % (THREADS / TILE) * 4;
-      static_assert(CHUNK / 4 <= THREADS / TILE, "sixteen threads a row take four numbers each");
-      if (t < wide) {
-        float4 v = *reinterpret_cast<const float4*>(part + row * PART + t);
+    if constexpr (TENSOR) {
+      first_product<TILE>(p, maps, (s * p.sections + sec0) * p.R, rows, 0, total, R16, rank, tn, sums);
+    } else {
+      for (int t0 = 0; t0 < total; t0 += CHUNK) {
+        first_product(p, a + (long long)sec0 * p.R * p.K, x, t0, total, R16, rank * WARPS + warp, part + warp * TILE * PART);
+        // the CTAs of the cluster run, and have read the sums of the sections before: their memory may be written
+        if (t0 == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        __syncthreads();
+        const int wide = min(CHUNK, total - t0);
+        const int row = threadIdx.x / (THREADS / TILE), t = threadIdx.x % (THREADS / TILE) * 4;
+        static_assert(CHUNK / 4 <= THREADS / TILE, "sixteen threads a row take four numbers each");
+        if (t < wide) {
+          float4 v = *reinterpret_cast<const float4*>(part + row * PART + t);
 #pragma unroll
-        for (int w = 1; w < WARPS; ++w) {
-          const float4 o = *reinterpret_cast<const float4*>(part + (w * TILE + row) * PART + t);
-          v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+          for (int w = 1; w < WARPS; ++w) {
+            const float4 o = *reinterpret_cast<const float4*>(part + (w * TILE + row) * PART + t);
+            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+          }
+          const uint32_t to = sm32(sums + (rank * TILE + row) * total + t0 + t);
+#pragma unroll
+          for (int c = 0; c < CLUSTER; ++c) st_cluster(to, c, v);
         }
-        const uint32_t to = sm32(sums + (rank * TILE + row) * total + t0 + t);
-#pragma unroll
-        for (int c = 0; c < CLUSTER; ++c) st_cluster(to, c, v);
+        __syncthreads();
       }
-      __syncthreads();
     }
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     // groups of 32 columns of one section, a warp each; the first ones are fetched while the cluster meets
     const int before = sec0 ? p.groups[sec0 - 1] : 0, groups = p.groups[sec1 - 1] - before, mine = (groups + CLUSTER - 1) / CLUSTER;
     const auto group = [&](Group<T, O>& gr, int i) {
-      int gi = rank * mine + i;
-      gr.s.sec = -1;
-      if (i < mine && gi < groups) {
-        gi += before;
-        gr.s = section_of_group(p, gi);
-        gr.u0 = gi * 32;
-      }
+      const int gi = rank * mine + i;
+      gr.gi = i < mine && gi < groups ? gi + before : -1;
       fetch(gr, p, b, base0, base1);
     };
     Group<T, O> ahead[AHEAD];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) group(ahead[i], warp + i * WARPS);
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    for (int row = threadIdx.x / (THREADS / TILE), t = threadIdx.x % (THREADS / TILE); t < total; t += THREADS / TILE) {
-      float v = 0.f;
+    if constexpr (TENSOR) {
+      for (int i = threadIdx.x; i < TILE * total; i += THREADS) {
+        const int row = i % TILE, t = i / TILE;
+        float v = 0.f;
 #pragma unroll
-      for (int c = 0; c < CLUSTER; ++c) v += sums[(c * TILE + row) * total + t];
-      keep_inner<SPLITS>(inner, total, row, t, v * scale);
+        for (int c = 0; c < CLUSTER; ++c) v += sums[(c * total + t) * SUM_ROW + row];
+        keep_inner<SPLITS>(inner, total, row, t, v * scale);
+      }
+    } else {
+      for (int row = threadIdx.x / (THREADS / TILE), t = threadIdx.x % (THREADS / TILE); t < total; t += THREADS / TILE) {
+        float v = 0.f;
+#pragma unroll
+        for (int c = 0; c < CLUSTER; ++c) v += sums[(c * TILE + row) * total + t];
+        keep_inner<SPLITS>(inner, total, row, t, v * scale);
+      }
     }
     __syncthreads();
     if (sec1 < p.sections) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-
     for (int i = warp; i < mine; i += AHEAD * WARPS) {
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         const Group<T, O> gr = ahead[j];
-        if (gr.s.sec < 0) continue;
+        if (gr.gi < 0) continue;
         group(ahead[j], i + (j + AHEAD) * WARPS);
         float acc[2][8];
-        second_product<SPLITS>(p, b, inner + (gr.s.sec - sec0) * R16, total, gr, R16, acc);
+        second_product<SPLITS>(p, b, inner, total, sec0, gr, R16, acc);
         if (gr.col >= 0 && out0) add_eight(gr.base[0], out0 + gr.col, acc[0]);
         if (gr.col >= 0 && out1) add_eight(gr.base[1], out1 + gr.col, acc[1]);
       }
     }
     __syncthreads();
   }
+  if constexpr (TENSOR) free_tensor(p, tn);
 }
 
-// ---- many rows, first kernel: the inner numbers of 64 rows by a cluster.  A warp multiplies 64 rows by 32 rows of A over its share of k
-// (x and A are each read once by a CTA); the eight warps' sums meet in shared memory, and CTA c of the cluster gets all of rows 8c .. 8c + 7.
-constexpr int WIDE_CHUNK = 32;
-constexpr int WIDE_PART = WIDE_CHUNK + 4;
-constexpr int SHARE = LIST / CLUSTER;
-
+// ---- many rows, first kernel: the inner numbers of 128 rows by a cluster, of which CTA c keeps rows 16c .. 16c + 15
 template <int SPLITS>
-__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) adapter_inner_kernel(const __grid_constant__ AdapterParams p) {
-  extern __shared__ __align__(16) float smem[];  // [WARPS][LIST][WIDE_PART] partial sums, then [CLUSTER][SHARE][total] sums
-  __shared__ long long offset[LIST];  // of the tile's rows in x (bytes), or -1
-  pdl_launch();
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) adapter_inner_kernel(const __grid_constant__ AdapterParams p, const __grid_constant__ Maps maps) {
+  extern __shared__ __align__(1024) float smem[];  // the ring of blocks, then the sums
+  __shared__ int rows[LIST];
+  __shared__ unsigned runs_of[LIST / 32];
+  __shared__ __align__(8) unsigned long long bars[BARS];
+  __shared__ uint32_t tmem_slot;
   pdl_wait();
   const int tile = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
   const int s = p.tiles[3 * tile], first = p.tiles[3 * tile + 1], count = p.tiles[3 * tile + 2];
-  if (s < 0 || count <= 0) return;
-  const int R = p.ranks ? min(max(p.ranks[s], 0), p.R) : p.R;
+  const int R = s < 0 || count <= 0 ? 0 : p.ranks ? min(max(p.ranks[s], 0), p.R) : p.R;
   if (R == 0) return;
-  if (threadIdx.x < LIST) offset[threadIdx.x] = threadIdx.x < count ? (long long)p.rows[first + threadIdx.x] * p.x_stride * 2 : -1;
-  __syncthreads();
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  const int R16 = (R + 15) & ~15, total = p.sections * R16;
-  const bf16* a = reinterpret_cast<const bf16*>(p.a) + (long long)s * p.sections * p.R * p.K;
-  const char* x = reinterpret_cast<const char*>(p.x);
-  float* sums = smem + WARPS * LIST * WIDE_PART;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  const int tall = (count + 15) / 16;  // sixteens of rows that there are
-  for (int t0 = 0; t0 < total; t0 += WIDE_CHUNK) {
-    float acc[4][4][4];
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
-    const bf16* rows[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = t0 + j * 8 + g, sec = (t >= R16) + (t >= 2 * R16) + (t >= 3 * R16);
-      rows[j] = t < total ? a + (long long)(sec * (p.R - R16) + t) * p.K : nullptr;
-    }
-    for (int k0 = (rank * WARPS + warp) * 32; k0 < p.K; k0 += 32 * CLUSTER * WARPS) {
-      const int k = k0 + q * 8;
-      const bool in = k < p.K;
-      uint4 w[4], lo[4], hi[4];
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const long long l = offset[m * 16 + g], h = offset[m * 16 + g + 8];
-        lo[m] = l >= 0 && in ? __ldg(reinterpret_cast<const uint4*>(x + l + 2ll * k)) : zero;
-        hi[m] = h >= 0 && in ? __ldg(reinterpret_cast<const uint4*>(x + h + 2ll * k)) : zero;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = rows[j] && in ? __ldg(reinterpret_cast<const uint4*>(rows[j] + k)) : zero;
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        if (m < tall) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mma(acc[m][j], lo[m].x, hi[m].x, lo[m].y, hi[m].y, w[j].x, w[j].y);
-            mma(acc[m][j], lo[m].z, hi[m].z, lo[m].w, hi[m].w, w[j].z, w[j].w);
-          }
-        }
-      }
-    }
-    if (t0) __syncthreads();  // the sums of the chunk before are read
-    float* part = smem + warp * LIST * WIDE_PART;
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        *reinterpret_cast<float2*>(part + (m * 16 + g) * WIDE_PART + j * 8 + 2 * q) = make_float2(acc[m][j][0], acc[m][j][1]);
-        *reinterpret_cast<float2*>(part + (m * 16 + g + 8) * WIDE_PART + j * 8 + 2 * q) = make_float2(acc[m][j][2], acc[m][j][3]);
-      }
-    if (t0 == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs of the cluster run: their memory may be written
-    __syncthreads();
-    // eight threads a row take four numbers each; rows 8c .. 8c + 7 go to CTA c
-#pragma unroll
-    for (int i = 0; i < LIST * 8 / THREADS; ++i) {
-      const int row = threadIdx.x / 8 + i * (THREADS / 8), t = threadIdx.x % 8 * 4;
-      if (row < count && t0 + t < total) {
-        float4 v = *reinterpret_cast<const float4*>(smem + row * WIDE_PART + t);
-#pragma unroll
-        for (int w = 1; w < WARPS; ++w) {
-          const float4 o = *reinterpret_cast<const float4*>(smem + (w * LIST + row) * WIDE_PART + t);
-          v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-        }
-        st_cluster(sm32(sums + (rank * SHARE + row % SHARE) * total + t0 + t), row / SHARE, v);
-      }
-    }
+  if (threadIdx.x < LIST) {
+    const int row = p.rows[first + (threadIdx.x < count ? threadIdx.x : 0)];  // (any row past the last: what comes of it is not read)
+    const bool run = __all_sync(0xffffffffu, row == __shfl_sync(0xffffffffu, row, 0) + (int)(threadIdx.x & 31));
+    rows[threadIdx.x] = row;
+    if ((threadIdx.x & 31) == 0) runs_of[threadIdx.x / 32] = run;
   }
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  Tensor tn = make_tensor(p, smem, bars, &tmem_slot);  // (a barrier)
+  pdl_launch();  // not before it has its tensor memory: a kernel that waits for this one could hold it
+  const unsigned runs = runs_of[0] | runs_of[1] << 1 | runs_of[2] << 2 | runs_of[3] << 3;
+  static_assert(LIST == 128, "four runs");
+  const int R16 = (R + 15) & ~15, together = min(p.sections, p.most / R16);
+  float* sums = reinterpret_cast<float*>(reinterpret_cast<char*>(smem) + p.slots * slot_bytes(LIST, p.most));
   const float scale = p.scales[s];
   const int wide = p.sections * p.R;  // numbers of a row of `inner`
-  bf16* inner = p.inner + (long long)tile * SPLITS * LIST * wide;
-  // a warp a row, two numbers a lane
-  const int row = rank * SHARE + warp;
-  if (row >= count) return;
-  for (int t = 2 * lane; t < total; t += 64) {
-    float v0 = 0.f, v1 = 0.f;
+  for (int sec0 = 0; sec0 < p.sections; sec0 += together) {
+    const int sec1 = min(p.sections, sec0 + together), total = (sec1 - sec0) * R16;
+    first_product<LIST>(p, maps, (s * p.sections + sec0) * p.R, rows, runs, total, R16, rank, tn, sums);
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // two neighbouring numbers of a row a thread
+    bf16* inner = p.inner + ((long long)tile * SPLITS * LIST + rank * TILE) * wide + sec0 * R16;
+    const int live = min(TILE, count - rank * TILE);
+    for (int i = threadIdx.x; i < TILE * (total / 2); i += THREADS) {
+      const int row = i / (total / 2), t = i % (total / 2) * 2;
+      if (row >= live) break;
+      float v0 = 0.f, v1 = 0.f;
 #pragma unroll
-    for (int c = 0; c < CLUSTER; ++c) {
-      const float2 v = *reinterpret_cast<const float2*>(sums + (c * SHARE + warp) * total + t);
-      v0 += v.x, v1 += v.y;
-    }
-    v0 *= scale, v1 *= scale;
+      for (int c = 0; c < CLUSTER; ++c) {
+        v0 += sums[(c * total + t) * SUM_ROW + row];
+        v1 += sums[(c * total + t + 1) * SUM_ROW + row];
+      }
+      v0 *= scale, v1 *= scale;
 #pragma unroll
-    for (int i = 0; i < SPLITS; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v0, v1);
-      *reinterpret_cast<__nv_bfloat162*>(inner + ((long long)i * LIST + row) * wide + t) = h;
-      const float2 f = __bfloat1622float2(h);
-      v0 = isinf(f.x) ? 0.f : v0 - f.x;
-      v1 = isinf(f.y) ? 0.f : v1 - f.y;
+      for (int k = 0; k < SPLITS; ++k) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v0, v1);
+        *reinterpret_cast<__nv_bfloat162*>(inner + ((long long)k * LIST + row) * wide + t) = h;
+        const float2 f = __bfloat1622float2(h);
+        v0 = isinf(f.x) ? 0.f : v0 - f.x;
+        v1 = isinf(f.y) ? 0.f : v1 - f.y;
+      }
     }
+    __syncthreads();
+    if (sec1 < p.sections) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
+  free_tensor(p, tn);
 }
 
-// ---- many rows, second kernel: 64 rows and 256 columns a CTA, 32 columns a warp
+// ---- many rows, second kernel: ROWS rows and `each` groups of 32 columns a warp, one after another; a group's pieces of the rows are fetched while
+// the group before is multiplied
+constexpr int ROWS = 64;
+
 template <typename O, int SPLITS>
-__global__ void __launch_bounds__(THREADS, 2) adapter_outer_kernel(const __grid_constant__ AdapterParams p) {
-  extern __shared__ __align__(16) bf16 held[];  // the tile's inner numbers: [SPLITS][LIST][stride]
-  __shared__ int rows[LIST];
+__global__ void __launch_bounds__(THREADS, 2) adapter_outer_kernel(const __grid_constant__ AdapterParams p, int each) {
+  extern __shared__ __align__(16) bf16 held[];  // the rows' inner numbers: [SPLITS][ROWS][stride]
+  __shared__ int rows[ROWS];
   pdl_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-  const int tile = blockIdx.y;
+  const int tile = blockIdx.y / (LIST / ROWS), r0 = blockIdx.y % (LIST / ROWS) * ROWS;
   pdl_wait();
-  const int s = p.tiles[3 * tile], first = p.tiles[3 * tile + 1], count = p.tiles[3 * tile + 2];
+  const int s = p.tiles[3 * tile], first = p.tiles[3 * tile + 1] + r0, count = min(ROWS, p.tiles[3 * tile + 2] - r0);
   if (count <= 0) return;
-  if (threadIdx.x < LIST) rows[threadIdx.x] = threadIdx.x < count ? p.rows[first + threadIdx.x] : -1;
+  if (threadIdx.x < ROWS) rows[threadIdx.x] = threadIdx.x < count ? p.rows[first + threadIdx.x] : -1;
   __syncthreads();
   const int R = s < 0 ? 0 : p.ranks ? min(max(p.ranks[s], 0), p.R) : p.R;
   if (R == 0) {
     copy_rows<O>(p, rows, count, blockIdx.x, gridDim.x);
     return;
   }
-  const int R16 = (R + 15) & ~15, total = p.sections * R16, wide = p.sections * p.R;
-  int gi = blockIdx.x * WARPS + warp;
-  const bool none = gi >= p.groups[MAX_SECTIONS - 1];
-  const Section sec = section_of_group(p, gi);
-  const int u = gi * 32 + 8 * q;
-  const int col = !none && u < sec.width ? column(p, sec, u) : -1;
+  const int R16 = (R + 15) & ~15, total = p.sections * R16, wide = p.sections * p.R, groups = p.groups[MAX_SECTIONS - 1];
+  const int stride = inner_stride(total, 2), tall = (count + 15) / 16;
   const bf16* b = reinterpret_cast<const bf16*>(p.b) + (long long)s * p.N * p.R;
-  const bf16* brow[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int ub = gi * 32 + (g >> 1) * 8 + 2 * j + (g & 1);
-    brow[j] = !none && ub < sec.width ? b + (long long)column(p, sec, ub) * p.R + 4 * q : nullptr;
-  }
-  // the rows that are added to and the first of B come while the inner numbers do
+
   constexpr int PIECES = sizeof(O) / 2;  // 16-byte pieces of eight columns
-  constexpr int EARLY = sizeof(O) == 2 ? 4 : 2;  // sixteens of rows whose pieces come early
-  uint4 base[4][2][PIECES];
-  const auto fetch = [&](int m) {
+  constexpr int HALVES = sizeof(O) == 2 ? 8 : 4;  // rows of a lane whose pieces are fetched a group ahead (of eight)
+  uint4 base[HALVES][PIECES];
+  Section sec{0, 0, 0};
+  int u0 = 0, col = -1;
+  uint2 w0[4];
+  const auto piece = [&](uint4 (&to)[PIECES], int h) {
+    const int r = rows[h * 8 + g];
+    if (r >= 0 && col >= 0) {
+      const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<const O*>(p.base) + r * p.base_stride + col);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = rows[m * 16 + h * 8 + g];
-      if (r >= 0 && col >= 0) {
-        const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<const O*>(p.base) + r * p.base_stride + col);
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) base[m][h][i] = at[i];
-      }
+      for (int i = 0; i < PIECES; ++i) to[i] = at[i];
     }
   };
+  const auto find = [&](int gi) {
+    sec = section_of_group(p, gi);
+    u0 = gi * 32;
+    col = u0 + 8 * q < sec.width ? column(p, sec, u0 + 8 * q) : -1;
 #pragma unroll
-  for (int m = 0; m < EARLY; ++m) fetch(m);
-  uint2 w0[4];
+    for (int j = 0; j < 4; ++j) {
+      const bf16* at = b_row(p, b, sec, u0, j);
+      w0[j] = at ? __ldg(reinterpret_cast<const uint2*>(at + 4 * q)) : make_uint2(0, 0);
+    }
+  };
+  int gi = blockIdx.x * each * WARPS + warp;
+  const int end = min(groups, (blockIdx.x + 1) * each * WARPS);
+  if (gi < end) {
+    find(gi);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w0[j] = brow[j] ? __ldg(reinterpret_cast<const uint2*>(brow[j])) : make_uint2(0, 0);
-  const int stride = inner_stride(total, 2), tall = (count + 15) / 16;
+    for (int h = 0; h < HALVES; ++h) piece(base[h], h);
+  }
   {
-    const bf16* inner = p.inner + (long long)tile * SPLITS * LIST * wide;
+    const bf16* inner = p.inner + ((long long)tile * SPLITS * LIST + r0) * wide;
     const int pieces = total / 8;
-    for (int r = threadIdx.x / 8; r < SPLITS * LIST; r += THREADS / 8) {
-      if (r % LIST >= tall * 16) continue;
-      const bool live = r % LIST < count;
-      for (int i = threadIdx.x % 8; i < pieces; i += 8)
-        *reinterpret_cast<uint4*>(held + r * stride + i * 8) = live ? *reinterpret_cast<const uint4*>(inner + (long long)r * wide + i * 8) : make_uint4(0, 0, 0, 0);
+    for (int r = threadIdx.x / 8; r < SPLITS * ROWS; r += THREADS / 8) {
+      const int row = r % ROWS;
+      if (row >= tall * 16) continue;
+      const bf16* from = inner + ((long long)(r / ROWS) * LIST + row) * wide;
+      for (int i = threadIdx.x % 8; i < pieces; i += 8) {
+        // (sections of an adapter of a lower rank lie close together)
+        *reinterpret_cast<uint4*>(held + r * stride + i * 8) = row < count ? *reinterpret_cast<const uint4*>(from + i * 8) : make_uint4(0, 0, 0, 0);
+      }
     }
   }
   __syncthreads();
-  if (none) return;
-  float acc[4][4][4];
+  for (; gi < end; gi += WARPS) {
+    const bf16* mine = held + g * stride + sec.sec * R16 + 4 * q;
+    const bool more = gi + WARPS < end;
+    // 32 rows at a time
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
+    for (int half = 0; half < 2; ++half) {
+      if (half * 2 >= tall) break;
+      float acc[2][4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
-  const bf16* mine = held + g * stride + sec.sec * R16 + 4 * q;
-  for (int r0 = 0; r0 < R16; r0 += 16) {
-    uint2 w[4], next[4];
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      w[j] = w0[j];
-      next[j] = r0 + 16 < R16 && brow[j] ? __ldg(reinterpret_cast<const uint2*>(brow[j] + r0 + 16)) : make_uint2(0, 0);
-    }
+          for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
+      for (int r = 0; r < R16; r += 16) {
+        uint2 w[4];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      if (m < tall) {
+        for (int j = 0; j < 4; ++j) {
+          w[j] = w0[j];
+          const bf16* at = r ? b_row(p, b, sec, u0, j) : nullptr;
+          if (r) w[j] = at ? __ldg(reinterpret_cast<const uint2*>(at + r + 4 * q)) : make_uint2(0, 0);
+        }
 #pragma unroll
-        for (int i = 0; i < SPLITS; ++i) {
-          const bf16* h = mine + (i * LIST + m * 16) * stride + r0;
-          const uint2 lo = *reinterpret_cast<const uint2*>(h), hi = *reinterpret_cast<const uint2*>(h + 8 * stride);
+        for (int m = 0; m < 2; ++m) {
+          if (half * 2 + m < tall) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mma(acc[m][j], lo.x, hi.x, lo.y, hi.y, w[j].x, w[j].y);
+            for (int i = 0; i < SPLITS; ++i) {
+              const bf16* h = mine + (i * ROWS + (half * 2 + m) * 16) * stride + r;
+              const uint2 lo = *reinterpret_cast<const uint2*>(h), hi = *reinterpret_cast<const uint2*>(h + 8 * stride);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) mma(acc[m][j], lo.x, hi.x, lo.y, hi.y, w[j].x, w[j].y);
+            }
+          }
         }
       }
-    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w0[j] = next[j];
+      for (int h = 0; h < 4; ++h) {
+        const int r = rows[half * 32 + h * 8 + g];
+        const int m = h / 2, e = h % 2 * 2;
+        const float v[8] = {acc[m][0][e], acc[m][0][e + 1], acc[m][1][e], acc[m][1][e + 1], acc[m][2][e], acc[m][2][e + 1], acc[m][3][e], acc[m][3][e + 1]};
+        if (r >= 0 && col >= 0) add_eight(base[(half * 4 + h) % HALVES], reinterpret_cast<O*>(p.out) + r * p.out_stride + col, v);
+        if (HALVES == 4 && half == 0) piece(base[h], 4 + h);
+      }
+    }
+    if (more) {
+      find(gi + WARPS);
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) piece(base[h], h);
+    }
   }
-#pragma unroll
-  for (int m = EARLY; m < 4; ++m) fetch(m);
-  if (col < 0) return;
-#pragma unroll
-  for (int m = 0; m < 4; ++m)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = rows[m * 16 + h * 8 + g];
-      if (r < 0) continue;
-      const float v[8] = {acc[m][0][2 * h], acc[m][0][2 * h + 1], acc[m][1][2 * h], acc[m][1][2 * h + 1], acc[m][2][2 * h], acc[m][2][2 * h + 1], acc[m][3][2 * h], acc[m][3][2 * h + 1]};
-      add_eight(base[m][h], reinterpret_cast<O*>(p.out) + r * p.out_stride + col, v);
-    }
+}
+
+// How many blocks of k shared memory holds, the columns of tensor memory; the bytes for the ring, the sums and the inner numbers (and 16 KB: the
+// last lanes of the accumulator read past the rows of A).
+size_t ring_smem(AdapterParams& p, int nr, int splits, size_t budget) {
+  const size_t rest = (size_t)CLUSTER * p.most * SUM_ROW * 4 + (nr == TILE ? (size_t)splits * TILE * (p.most + 16) * 2 : 0) + 16 * 1024, slot = slot_bytes(nr, p.most);
+  const int blocks = ((p.K + BLOCK_K - 1) / BLOCK_K + CLUSTER - 1) / CLUSTER;
+  p.slots = (int)(budget > rest ? (budget - rest) / slot : 0);
+  p.slots = max(1, min(min(p.slots, MAX_SLOTS), blocks));
+  p.tmem = 32;
+  while (p.tmem < (p.most + 127) / 128 * nr) p.tmem *= 2;
+  return p.slots * slot + rest;
+}
+
+// x: [n][K], one row a box and 32; A: [S sections R][K], sixteen rows a box; zeros past K
+int make_maps(const AdapterParams& p, Maps& maps) {
+  tc::EncodeTiledFn fn = tc::encode_tiled();
+  if (!fn) return (int)cudaErrorNotSupported;
+  const cuuint32_t ones[2] = {1, 1};
+  const auto encode = [&](CUtensorMap* map, const void* at, long long rows, long long stride, int box_rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)p.K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)BLOCK_K, (cuuint32_t)box_rows};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(at), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  return encode(&maps.x, p.x, p.n, p.x_stride, 1) && encode(&maps.run, p.x, p.n, p.x_stride, 32) && encode(&maps.a, p.a, (long long)p.S * p.sections * p.R, p.K, 16) ? 0 : (int)cudaErrorInvalidValue;
 }
 
 template <typename O, int SPLITS>
-int run_wide(const AdapterParams& p, int tiles, cudaStream_t st) {
-  const int total = p.sections * p.R;
-  const size_t one = (size_t)(WARPS * LIST * WIDE_PART + CLUSTER * SHARE * total) * 4, two = (size_t)SPLITS * LIST * inner_stride(total, 2) * 2;
+int run_wide(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
+  const int total = p.sections * p.R, groups = p.groups[MAX_SECTIONS - 1];
+  const size_t one = ring_smem(p, LIST, SPLITS, 220 * 1024), two = (size_t)SPLITS * ROWS * inner_stride(total, 2) * 2;
   const auto inner = adapter_inner_kernel<SPLITS>;
   const auto outer = adapter_outer_kernel<O, SPLITS>;
   cudaError_t rc = cudaFuncSetAttribute(inner, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one);
   if (rc == cudaSuccess) rc = cudaFuncSetAttribute(outer, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)two);
   if (rc != cudaSuccess) return (int)rc;
-  const int r = launch(inner, dim3(tiles * CLUSTER), dim3(THREADS), one, st, p);
+  const int r = launch(inner, dim3(tiles * CLUSTER), dim3(THREADS), one, st, p, maps);
   if (r) return r;
-  return launch(outer, dim3((p.groups[MAX_SECTIONS - 1] + WARPS - 1) / WARPS, tiles), dim3(THREADS), two, st, p);
+  // groups a warp: as many as leave about two CTAs for every SM
+  const int stripes = (groups + WARPS - 1) / WARPS, blocks = (p.n + ROWS - 1) / ROWS;
+  const int each = max(1, min(8, (int)((long long)stripes * blocks / (2 * 148))));
+  return launch(outer, dim3((stripes + each - 1) / each, tiles * (LIST / ROWS)), dim3(THREADS), two, st, p, each);
 }
 
-// ---- the rows of a step by adapter: one CTA.  Rows without an adapter come last.
+// ---- the rows of a step by adapter: one CTA.  Rows without an adapter come last.  The rows of an adapter keep their order within a
+// warp's 32; whoever places the first row of a tile writes the tile.
 constexpr int SORT = 1024;
 __global__ void __launch_bounds__(SORT) adapter_group_kernel(const int* __restrict__ ids, int n, int S, int tile, int max_tiles, int* __restrict__ rows, int* __restrict__ tiles,
                                                              int* __restrict__ err) {
   pdl_launch();
   pdl_wait();
-  extern __shared__ int count[];  // [S + 1] rows, then [S + 1] where they begin
+  extern __shared__ int count[];  // [S + 1] rows, then [S + 1] where they and [S + 1] where their tiles begin, then [S + 1] how many are placed
   int* from = count + S + 1;
+  int* tile0 = from + S + 1;
+  int* placed = tile0 + S + 1;
   __shared__ int warp_rows[32], warp_tiles[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i <= S; i += SORT) count[i] = 0;
-  __syncthreads();
+  for (int i = threadIdx.x; i <= S; i += SORT) count[i] = placed[i] = 0;
   const int rounds = (n + SORT - 1) / SORT;
+  constexpr int KEPT = 4;  // rounds whose ids stay in registers
+  int kept[KEPT];
+#pragma unroll
+  for (int r = 0; r < KEPT; ++r) kept[r] = r * SORT + (int)threadIdx.x < n ? ids[r * SORT + threadIdx.x] : -2;
+  const auto check = [&](int raw, int i) {
+    if (i < n && (raw < -1 || raw >= S) && err) atomicOr(err, 32);
+    return i >= n ? -2 : raw >= 0 && raw < S ? raw : S;
+  };
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < KEPT; ++r) kept[r] = check(kept[r], r * SORT + threadIdx.x);
   for (int r = 0; r < rounds; ++r) {
     const int i = r * SORT + threadIdx.x;
-    int s = i < n ? valid_id(ids[i], S, err) : -2;
-    if (s == -1) s = S;
+    const int s = r == 0 ? kept[0] : r == 1 ? kept[1] : r == 2 ? kept[2] : r == 3 ? kept[3] : check(i < n ? ids[i] : -2, i);
     const unsigned same = __match_any_sync(0xffffffffu, s);
     if (s >= 0 && lane == __ffs(same) - 1) atomicAdd(&count[s], __popc(same));
   }
@@ -758,44 +897,48 @@ __global__ void __launch_bounds__(SORT) adapter_group_kernel(const int* __restri
   }
   if (lane == 31) warp_rows[warp] = rs, warp_tiles[warp] = ts;
   __syncthreads();
-  int r0 = rs - rows_here, t0 = ts - tiles_here, all = 0;
-  for (int w = 0; w < SORT / 32; ++w) {
-    if (w < warp) r0 += warp_rows[w], t0 += warp_tiles[w];
-    all += warp_tiles[w];
+  // (the warps' sums, scanned by every warp for itself)
+  int wr = warp_rows[lane], wt = warp_tiles[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int r = __shfl_up_sync(0xffffffffu, wr, o), t = __shfl_up_sync(0xffffffffu, wt, o);
+    if (lane >= o) wr += r, wt += t;
   }
+  const int all = __shfl_sync(0xffffffffu, wt, 31);
+  const int wr0 = __shfl_sync(0xffffffffu, wr, max(warp - 1, 0)), wt0 = __shfl_sync(0xffffffffu, wt, max(warp - 1, 0));
+  int r0 = rs - rows_here + (warp ? wr0 : 0), t0 = ts - tiles_here + (warp ? wt0 : 0);
   for (int i = lo; i < hi; ++i) {
-    from[i] = r0;
-    for (int at = 0; at < count[i]; at += tile, ++t0) {
-      tiles[3 * t0] = i == S ? -1 : i;
-      tiles[3 * t0 + 1] = r0 + at;
-      tiles[3 * t0 + 2] = min(tile, count[i] - at);
-    }
-    r0 += count[i];
+    from[i] = r0, tile0[i] = t0;
+    r0 += count[i], t0 += (count[i] + tile - 1) / tile;
   }
   for (int i = all + threadIdx.x; i < max_tiles; i += SORT) tiles[3 * i] = -1, tiles[3 * i + 1] = 0, tiles[3 * i + 2] = 0;
   __syncthreads();
   for (int r = 0; r < rounds; ++r) {
     const int i = r * SORT + threadIdx.x;
-    int s = i < n ? valid_id(ids[i], S, nullptr) : -2;
-    if (s == -1) s = S;
+    const int s = r == 0 ? kept[0] : r == 1 ? kept[1] : r == 2 ? kept[2] : r == 3 ? kept[3] : check(i < n ? ids[i] : -2, i);
     const unsigned same = __match_any_sync(0xffffffffu, s);
-    const int first = __ffs(same) - 1;
+    const int leader = __ffs(same) - 1;
     int at = 0;
-    if (s >= 0 && lane == first) at = atomicAdd(&from[s], __popc(same));
-    at = __shfl_sync(0xffffffffu, at, first);
-    if (s >= 0) rows[at + __popc(same & ((1u << lane) - 1))] = i;
+    if (s >= 0 && lane == leader) at = atomicAdd(&placed[s], __popc(same));
+    at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1));
+    if (s >= 0) {
+      rows[from[s] + at] = i;
+      if (at % tile == 0) {
+        int* t = tiles + 3 * (tile0[s] + at / tile);
+        t[0] = s == S ? -1 : s, t[1] = from[s] + at, t[2] = min(tile, count[s] - at);
+      }
+    }
   }
 }
 
 template <typename T, typename O, int SPLITS>
-int run_tiles(const AdapterParams& p, int tiles, cudaStream_t st) {
-  static_assert(3 * TILE * (MOST + 16) * 2 <= WARPS * TILE * PART * 4 && TILE * (MOST + 4) * 4 <= WARPS * TILE * PART * 4, "the numbers between the products take the partial sums' place");
-  const int total = min(p.sections * p.R, MOST);
-  const size_t smem = (size_t)(WARPS * TILE * PART + CLUSTER * TILE * total) * 4;
+int run_tiles(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
+  static_assert(TILE * (MOST + 4) * 4 <= WARPS * TILE * PART * 4, "the inner numbers take the partial sums' place");
+  const size_t smem = sizeof(T) == 2 ? ring_smem(p, TILE, SPLITS, 112 * 1024) : (size_t)(WARPS * TILE * PART + CLUSTER * TILE * p.most) * 4;
   const auto kernel = adapter_tile_kernel<T, O, SPLITS>;
   const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (rc != cudaSuccess) return (int)rc;
-  return launch(kernel, dim3(tiles * CLUSTER), dim3(THREADS), smem, st, p);
+  return launch(kernel, dim3(tiles * CLUSTER), dim3(THREADS), smem, st, p, maps);
 }
 
 }  // namespace
@@ -807,8 +950,12 @@ KVF_API int kvf_adapters_set_pdl(int on) {
 
 KVF_API int kvf_adapter_group(const int* ids, int n, int S, int tile, int max_tiles, int* rows, int* tiles, int* err, cudaStream_t st) {
   if (n <= 0) return 0;
-  const size_t smem = (size_t)2 * (S + 1) * sizeof(int);
-  if (smem > 40 * 1024) return (int)cudaErrorInvalidValue;
+  const size_t smem = (size_t)4 * (S + 1) * sizeof(int);
+  if (smem > 96 * 1024) return (int)cudaErrorInvalidValue;
+  if (smem > 40 * 1024) {
+    const cudaError_t rc = cudaFuncSetAttribute(adapter_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (rc != cudaSuccess) return (int)rc;
+  }
   return launch(adapter_group_kernel, dim3(1), dim3(SORT), smem, st, ids, n, S, tile, max_tiles, rows, tiles, err);
 }
 
@@ -825,12 +972,16 @@ int run(AdapterParams& p, const int* ends, int wide, int max_tiles, int two, cud
     p.groups[i] = (i ? p.groups[i - 1] : 0) + (p.width[i] + 31) / 32;
     from = end;
   }
+  p.most = min(p.sections, MOST / p.R) * p.R;
+  Maps maps;
   if constexpr (sizeof(T) == 2) {
-    if (two && p.tiles && p.inner && max_tiles <= 65535) return wide ? run_wide<float, 3>(p, max_tiles, st) : run_wide<bf16, 2>(p, max_tiles, st);
+    const int rc = make_maps(p, maps);
+    if (rc) return rc;
+    if (two && p.tiles && p.inner && max_tiles <= 65535) return wide ? run_wide<float, 3>(p, maps, max_tiles, st) : run_wide<bf16, 2>(p, maps, max_tiles, st);
   }
   const int tiles = p.tiles ? max_tiles * (LIST / TILE) : p.n;
-  if (wide) return run_tiles<T, float, WIDE_SPLITS>(p, tiles, st);
-  return run_tiles<T, T, sizeof(T) == 2 ? 2 : 1>(p, tiles, st);
+  if (wide) return run_tiles<T, float, WIDE_SPLITS>(p, maps, tiles, st);
+  return run_tiles<T, T, sizeof(T) == 2 ? 2 : 1>(p, maps, tiles, st);
 }
 
 }  // namespace
@@ -839,7 +990,7 @@ int run(AdapterParams& p, const int* ends, int wide, int max_tiles, int two, cud
   KVF_API int kvf_adapter_add_##SUF(const void* x, long long x_stride, const void* a, const void* b, const float* scales, const int* ranks, const int* ids, int n, int S,  \
                                     int sections, int R, int K, int N, int end0, int end1, int end2, int alternating, const void* base, long long base_stride, void* out,  \
                                     long long out_stride, int wide, const int* rows, const int* tiles, int max_tiles, void* inner, int two, int* err, cudaStream_t st) {   \
-    AdapterParams p{x, a, b, scales, ranks, ids, rows, tiles, (bf16*)inner, base, out, err, x_stride, base_stride, out_stride, n, S, sections, R, K, N, {}, {}, {}, alternating}; \
+    AdapterParams p{x, a, b, scales, ranks, ids, rows, tiles, (bf16*)inner, base, out, err, x_stride, base_stride, out_stride, n, S, sections, R, K, N, {}, {}, {}, alternating, 0, 0, 0}; \
     const int ends[3] = {end0, end1, end2};                                                                                                                               \
     return run<T, WIDE_SPLITS>(p, ends, wide, max_tiles, two, st);                                                                                                             \
   }

@@ -2883,7 +2883,7 @@ class AdapterBank:
 
 ADAPTER_DIRECT = 64  # up to so many rows the kernels group for themselves
 ADAPTER_MANY = 256  # from so many bfloat16 rows on the two products are kernels of their own
-ADAPTER_TILE = 64  # rows of one adapter that a tile of the list has room for
+ADAPTER_TILE = 128  # rows of one adapter that a tile of the list has room for
 
 
 class AdapterGroups:
