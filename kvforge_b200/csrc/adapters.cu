@@ -32,8 +32,7 @@ constexpr int CLUSTER = 8;      // CTAs a tile
 constexpr int DIRECT = 64;      // up to so many rows are grouped by every cluster itself
 constexpr int CHUNK = 48;       // rows of A a warp multiplies at a time
 constexpr int PART = CHUNK + 4; // floats from one row of the partial sums to the next
-constexpr int AHEAD = 2;        // groups of columns that a warp fetches ahead
-constexpr int MOST = 192;       // numbers between the products of a row that are in shared memory at a time (whole sections)
+constexpr int MOST = 128;       // numbers between the products of a row that are in shared memory at a time (whole sections)
 
 struct AdapterParams {
   const void* x;
@@ -54,7 +53,8 @@ struct AdapterParams {
   int begin[MAX_SECTIONS], width[MAX_SECTIONS], groups[MAX_SECTIONS];
   int alternating;
   int most;   // inner numbers of a row that shared memory holds at a time (whole sections of rank R)
-  int slots;  // blocks of 64 columns of k that it holds (bf16)
+  int stage;  // bytes of shared memory that columns of B and of the rows take in turn (few rows)
+  int slots;  // blocks of 64 columns of k that it holds (of a warp, where there are few rows; bf16)
   int tmem;   // columns of tensor memory
 };
 
@@ -63,9 +63,15 @@ struct AdapterParams {
 struct Section {
   int sec, begin, width;
 };
-// The section of group `gi` of 32 columns; gi becomes its number there.
+// The section of group `gi` of 32 columns; gi becomes its number there.  Alternating sections take turns, so that groups that follow one another
+// lie side by side.
 __device__ __forceinline__ Section section_of_group(const AdapterParams& p, int& gi) {
   Section s{0, p.begin[0], p.width[0]};
+  if (p.alternating) {
+    s.sec = gi & 1;
+    gi >>= 1;
+    return s;
+  }
   int before = 0;
 #pragma unroll
   for (int i = 1; i < MAX_SECTIONS; ++i)
@@ -102,7 +108,7 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
                :
                : "memory");
 }
-__device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+__device__ __forceinline__ void prefetch_map(const void* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory"); }
 
 // Column of the result that is number u of a section.
 __device__ __forceinline__ int column(const AdapterParams& p, const Section& s, int u) { return p.alternating ? (u >> 3) * 16 + s.sec * 8 + (u & 7) : s.begin + u; }
@@ -160,15 +166,11 @@ __device__ __forceinline__ void first_product(const AdapterParams& p, const floa
 constexpr int BLOCK_K = 64;  // columns of a block: a 128-byte row of the swizzled tiles
 constexpr int MAX_SLOTS = WARPS - 1;  // (a slot has a warp of its own that fills it)
 constexpr int BARS = 2 * MAX_SLOTS + 1;
+constexpr int FEW_SLOTS = 2;  // of a warp
 constexpr int SUM_ROW = 20;  // floats from the sums of one row of A to the next's: of 16 rows of x, and room against bank conflicts
 
 struct Maps {
-  CUtensorMap x, run, a;  // rows of x, twice, and of all adapters' A, 64 columns a box: one row, 32 rows, sixteen rows
-};
-
-struct Tensor {
-  uint32_t ring, bars, tmem;  // blocks ([NR rows of x | rows of A] each); barriers: a slot is filled, its products are done, all are; accumulator
-  int block, pass;            // blocks and passes so far: what phase the barriers are in
+  CUtensorMap x, run, a, whole;  // rows of x, twice, and of all adapters' A, twice, 64 columns a box: one row, 32 rows; sixteen rows, `most`
 };
 
 __host__ __device__ constexpr int slot_bytes(int nr, int rows) { return (nr + rows) * BLOCK_K * 2; }
@@ -180,17 +182,98 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// This CTA's share of a[total rows][k] x[NR rows][k], sent to where it is needed: the sums of `sums[rank][t][SUM_ROW]`, of all 16 rows in every CTA of
-// the cluster (NR = 16), or of rows 16c .. 16c + 15 in CTA c (NR = 128).  a0: the first of the sections' rows of A among all adapters'; rows:
+// Few rows: a warp fetches blocks of its own, waits for them and multiplies them (a tcgen05 product of 128 x 16 x 16 takes 128 cycles for its
+// operand A alone: 4,100 for 512 columns of k, where eight warps of mma.sync take some 300).  Block j of the CTA is warp j % 8's.
+struct Few {
+  uint32_t ring, bar;  // the warp's slots ([16 rows of x | rows of A] each) and their barriers
+  int block;           // blocks so far
+};
+
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+// The warp's share of x[16 rows][k] a[total rows][k] into part[16][total + 4] (in its first slot).
+__device__ __forceinline__ void first_product(const AdapterParams& p, const Maps& maps, int a0, const int* rows, int total, int R16, int rank, Few& few, float* part) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int every = (p.K + BLOCK_K - 1) / BLOCK_K, all = (every - rank + CLUSTER - 1) / CLUSTER;  // the CTA's blocks
+  const int blocks = (all - warp + WARPS - 1) / WARPS;                                           // the warp's (none for some where K is short)
+  const uint32_t bytes = slot_bytes(TILE, total);
+  const bool whole = R16 == p.R && total == p.most;
+  const auto load = [&](int j) {
+    const int slot = (few.block + j) % p.slots;
+    const uint32_t to = few.ring + slot * slot_bytes(TILE, p.most), bar = few.bar + 8 * slot;
+    const int k = (rank + CLUSTER * (warp + WARPS * j)) * BLOCK_K;
+    tc::bar_expect_tx(bar, bytes);
+    if (whole) tc::tma_load_2d(to + TILE * 128, &maps.whole, k, a0, bar);
+    for (int t = whole ? total : 0, sec = 0, in = 0; t < total; t += 16) {
+      tc::tma_load_2d(to + (TILE + t) * 128, &maps.a, k, a0 + sec * p.R + in, bar);
+      in += 16;
+      if (in == R16) in = 0, ++sec;
+    }
+#pragma unroll
+    for (int r = 0; r < TILE; r += 4) tma_gather4(to + r * 128, &maps.x, k, rows[r], rows[r + 1], rows[r + 2], rows[r + 3], bar);
+  };
+  if (elect_one())
+    for (int j = 0; j < min(blocks, p.slots); ++j) load(j);
+  __syncwarp();
+  float acc[MOST / 8][4];
+#pragma unroll
+  for (int j = 0; j < MOST / 8; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+  // lane l names row l % 16 of a 16 x 16 piece, columns 8 (l / 16) on
+  const int lr = lane & 15, lc = lane >> 4;
+  for (int j = 0; j < blocks; ++j) {
+    const int slot = (few.block + j) % p.slots, turn = (few.block + j) / p.slots;
+    const uint32_t at = few.ring + slot * slot_bytes(TILE, p.most);
+    tc::bar_wait(few.bar + 8 * slot, turn & 1, p.err);
+#pragma unroll
+    for (int i = 0; i < BLOCK_K / 16; ++i) {
+      uint32_t x[4];
+      ldsm_x4(x, at + tc::sw128(lr, 2 * i + lc));
+#pragma unroll
+      for (int t = 0; t < MOST / 16; ++t) {
+        if (t * 16 < total) {
+          uint32_t w[4];
+          ldsm_x4(w, at + tc::sw128(TILE + t * 16 + lr, 2 * i + lc));
+          mma(acc[2 * t], x[0], x[1], x[2], x[3], w[0], w[2]);
+          mma(acc[2 * t + 1], x[0], x[1], x[2], x[3], w[1], w[3]);
+        }
+      }
+    }
+    __syncwarp();
+    if (j + p.slots < blocks && elect_one()) load(j + p.slots);
+    __syncwarp();
+  }
+  few.block += max(blocks, 0);
+#pragma unroll
+  for (int j = 0; j < MOST / 8; ++j) {
+    if (j * 8 < total) {
+      *reinterpret_cast<float2*>(part + g * (total + 4) + j * 8 + 2 * q) = make_float2(acc[j][0], acc[j][1]);
+      *reinterpret_cast<float2*>(part + (g + 8) * (total + 4) + j * 8 + 2 * q) = make_float2(acc[j][2], acc[j][3]);
+    }
+  }
+}
+
+struct Tensor {
+  uint32_t ring, bars, tmem;  // blocks ([NR rows of x | rows of A] each); barriers: a slot is filled, its products are done, all are; accumulator
+  int block, pass;            // blocks and passes so far: what phase the barriers are in
+};
+
+
+
+// Many rows: this CTA's share of a[total rows][k] x[128 rows][k], sent to where it is needed: CTA c of the cluster gets the sums of rows
+// 16c .. 16c + 15 of x, in `sums[rank][t][SUM_ROW]`.  a0: the first of the sections' rows of A among all adapters'; rows:
 // of x, each valid; runs: bit i, rows 32i .. 32i + 31 follow one another in x.  Blocks are the cluster's in turn: block j of the CTA is block
-// rank + 8 j of k.  Warp 0 multiplies; a block is fetched by one thread of another warp (a warp takes some 90 cycles for each copy that it
-// starts: all of eight blocks by one warp kept eight rows and 4096 columns waiting for 5,700 cycles).
-template <int NR>
+// rank + 8 j of k.  Warp 0 multiplies; a slot is filled by a thread of a warp of its own (a warp takes some 90 cycles for each copy that it starts).
 __device__ __forceinline__ void first_product(const AdapterParams& p, const Maps& maps, int a0, const int* rows, unsigned runs, int total, int R16, int rank, Tensor& tn, float* sums) {
+  constexpr int NR = LIST;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int every = (p.K + BLOCK_K - 1) / BLOCK_K, blocks = (every - rank + CLUSTER - 1) / CLUSTER;  // (none for some where K is short)
   const uint32_t bytes = slot_bytes(NR, total), filled = tn.bars, done = filled + 8 * MAX_SLOTS, all = done + 8 * MAX_SLOTS;
   const int tiles = (total + 127) / 128;
+  const bool whole = R16 == p.R && total == p.most;
   if (warp > 0) {
     // Warp w fills slot w - 1 and no other, one block after another: what it waits for is never more than one phase ahead of the barrier
     // (a parity tells only two neighbouring phases apart).
@@ -202,7 +285,8 @@ __device__ __forceinline__ void first_product(const AdapterParams& p, const Maps
         const uint32_t to = tn.ring + slot * bytes, bar = filled + 8 * slot;
         tc::bar_expect_tx(bar, bytes);
         const int k = (rank + CLUSTER * j) * BLOCK_K;
-        for (int t = 0, sec = 0, in = 0; t < total; t += 16) {
+        if (whole) tc::tma_load_2d(to + NR * 128, &maps.whole, k, a0, bar);
+        for (int t = whole ? total : 0, sec = 0, in = 0; t < total; t += 16) {
           tc::tma_load_2d(to + (NR + t) * 128, &maps.a, k, a0 + sec * p.R + in, bar);
           in += 16;
           if (in == R16) in = 0, ++sec;
@@ -253,17 +337,11 @@ __device__ __forceinline__ void first_product(const AdapterParams& p, const Maps
     const uint32_t from = tn.tmem + m * NR + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t to = sm32(sums + (rank * total + t + lane) * SUM_ROW);
     uint32_t r[16];
-    if (NR == 16) {
-      tmem_ld16(from, r);
-      tmem_wait16(r);
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int cta = (warp >> 2) * 4 + i;
-      if (NR != 16) {
-        tmem_ld16(from + cta * 16, r);
-        tmem_wait16(r);
-      }
+      tmem_ld16(from + cta * 16, r);
+      tmem_wait16(r);
       if (t + lane < total) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -316,72 +394,32 @@ __device__ __forceinline__ void keep_inner(float* inner, int total, int row, int
   inner[row * inner_stride(total, 4) + t] = v;
 }
 
-// Where a group of 32 columns of a section lies for a lane, and what of it can be fetched before the inner numbers are there: the first
-// sixteen numbers of its rows of B (bf16) and the rows that are added to.
-template <typename T, typename O>
-struct Group {
-  int gi;        // its number, or -1
-  int col;       // the lane's first column of the result, or -1
-  uint2 w[4];    // bf16: B
-  uint4 base[2][sizeof(O) / 2];
-};
-
-// Row of B for the lane's column of the j-th of four tensor-core tiles: column 2q + e of it is column 8q + 2j + e of the 32, so that a lane's
-// eight results lie side by side.
-__device__ __forceinline__ const bf16* b_row(const AdapterParams& p, const bf16* b, const Section& s, int u0, int j) {
-  const int g = (threadIdx.x & 31) >> 2, u = u0 + (g >> 1) * 8 + 2 * j + (g & 1);
-  return u < s.width ? b + (long long)column(p, s, u) * p.R : nullptr;
-}
-
-template <typename T, typename O>
-__device__ __forceinline__ void fetch(Group<T, O>& gr, const AdapterParams& p, const T* b, const O* base0, const O* base1) {
-  const int q = threadIdx.x & 3;
-  gr.col = -1;
-  if (gr.gi < 0) return;
-  int gi = gr.gi;
-  const Section s = section_of_group(p, gi);
-  const int u = gi * 32 + 8 * q;
-  if (u < s.width) gr.col = column(p, s, u);
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const T* row = b_row(p, b, s, gi * 32, j);
-      gr.w[j] = row ? __ldg(reinterpret_cast<const uint2*>(row + 4 * q)) : make_uint2(0, 0);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(O) / 2; ++i) {
-    if (gr.col >= 0 && base0) gr.base[0][i] = *(reinterpret_cast<const uint4*>(base0 + gr.col) + i);
-    if (gr.col >= 0 && base1) gr.base[1][i] = *(reinterpret_cast<const uint4*>(base1 + gr.col) + i);
-  }
-}
-
-// acc[row half][column]: eight columns a lane; sec0: the section that `inner` begins with
-template <int SPLITS, typename O>
-__device__ __forceinline__ void second_product(const AdapterParams& p, const bf16* b, const bf16* inner, int total, int sec0, const Group<bf16, O>& gr, int R16, float (&acc)[2][8]) {
+// A group of 32 columns of a section: its own 16 numbers a row of B ... in shared memory (`b`, from column `c0` on) and the inner numbers make
+// acc[row half][column], eight columns a lane.
+// Column 2q + e of the j-th of four tensor-core tiles is column 8q + 2j + e of the 32, so that a lane's eight results lie side by side.
+template <int SPLITS>
+__device__ __forceinline__ void second_product(const AdapterParams& p, const bf16* b, int c0, const bf16* inner, int total, const Section& s, int u0, int R16, float (&acc)[2][8]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int stride = inner_stride(total, 2);
-  int gi = gr.gi;
-  const Section s = section_of_group(p, gi);
+  const bf16* rows[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int u = min(u0 + (g >> 1) * 8 + 2 * j + (g & 1), s.width - 1);  // (columns past the section's are not written)
+    rows[j] = b + (column(p, s, u) - c0) * p.R + 4 * q;
+  }
   float c[4][4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
-  const bf16* mine = inner + g * stride + (s.sec - sec0) * R16 + 4 * q;
-  for (int r0 = 0; r0 < R16; r0 += 16) {
+  const bf16* mine = inner + g * stride + 4 * q;
+  for (int r = 0; r < R16; r += 16) {
     uint2 w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      w[j] = gr.w[j];
-      if (r0) {
-        const bf16* row = b_row(p, b, s, gi * 32, j);
-        w[j] = row ? __ldg(reinterpret_cast<const uint2*>(row + r0 + 4 * q)) : make_uint2(0, 0);
-      }
-    }
+    for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint2*>(rows[j] + r);
 #pragma unroll
     for (int i = 0; i < SPLITS; ++i) {
-      const bf16* h = mine + i * TILE * stride + r0;
+      const bf16* h = mine + i * TILE * stride + r;
       const uint2 lo = *reinterpret_cast<const uint2*>(h), hi = *reinterpret_cast<const uint2*>(h + 8 * stride);
 #pragma unroll
       for (int j = 0; j < 4; ++j) mma(c[j], lo.x, hi.x, lo.y, hi.y, w[j].x, w[j].y);
@@ -394,27 +432,35 @@ __device__ __forceinline__ void second_product(const AdapterParams& p, const bf1
   }
 }
 
-template <int SPLITS, typename O>
-__device__ __forceinline__ void second_product(const AdapterParams& p, const float* b, const float* inner, int total, int sec0, const Group<float, O>& gr, int R16, float (&acc)[2][8]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2;
+template <int SPLITS>
+__device__ __forceinline__ void second_product(const AdapterParams& p, const float* b, int c0, const float* inner, int total, const Section& s, int u0, int R16, float (&acc)[2][8]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int stride = inner_stride(total, 4);
-  int gi = gr.gi;
-  const Section s = section_of_group(p, gi);
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[0][i] = acc[1][i] = 0.f;
-  if (gr.col < 0) return;
-  const float* rows = b + (long long)gr.col * p.R;
-  const float* lo = inner + g * stride + (s.sec - sec0) * R16;
+  if (u0 + 8 * q >= s.width) return;
+  const float* rows = b + (column(p, s, u0 + 8 * q) - c0) * p.R;
+  const float* lo = inner + g * stride;
   const float* hi = lo + 8 * stride;
   for (int r = 0; r < R16; r += 4) {
     const float4 l = *reinterpret_cast<const float4*>(lo + r), h = *reinterpret_cast<const float4*>(hi + r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float4 w = __ldg(reinterpret_cast<const float4*>(rows + (long long)i * p.R + r));
+      const float4 w = *reinterpret_cast<const float4*>(rows + i * p.R + r);
       acc[0][i] = fmaf(w.w, l.w, fmaf(w.z, l.z, fmaf(w.y, l.y, fmaf(w.x, l.x, acc[0][i]))));
       acc[1][i] = fmaf(w.w, h.w, fmaf(w.z, h.z, fmaf(w.y, h.y, fmaf(w.x, h.x, acc[1][i]))));
     }
   }
+}
+
+// Row of B (in memory) for the lane's column of the j-th tensor-core tile.
+__device__ __forceinline__ const bf16* b_row(const AdapterParams& p, const bf16* b, const Section& s, int u0, int j) {
+  const int g = (threadIdx.x & 31) >> 2, u = u0 + (g >> 1) * 8 + 2 * j + (g & 1);
+  return u < s.width ? b + (long long)column(p, s, u) * p.R : nullptr;
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
 // eight columns of a row: what they were and what is added
@@ -478,6 +524,8 @@ __device__ __forceinline__ int own_rows(const AdapterParams& p, int t, int* rows
   if (threadIdx.x < 32) {
     if (a == s && ra >= before && ra < before + TILE) rows[ra - before] = lane;
     if (b == s && rb >= before && rb < before + TILE) rows[rb - before] = lane + 32;
+    __syncwarp();
+    if (lane >= count && lane < TILE) rows[lane] = rows[0];  // (what comes of them is not read)
   }
   return count;
 }
@@ -485,13 +533,16 @@ __device__ __forceinline__ int own_rows(const AdapterParams& p, int t, int* rows
 // T: type of x, A and B; O: of base and out
 template <typename T, typename O, int SPLITS>
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) adapter_tile_kernel(const __grid_constant__ AdapterParams p, const __grid_constant__ Maps maps) {
-  // float32: the warps' partial sums (whose place the inner numbers take), then the CTAs' sums.  bfloat16: the ring of blocks, the sums, the inner numbers.
+  // the warps' blocks (bfloat16) or partial sums (float32), whose place columns of B and of the rows take later; the CTAs' sums; the inner numbers
   extern __shared__ __align__(1024) float smem[];
   __shared__ int rows[TILE];
-  __shared__ __align__(8) unsigned long long bars[BARS];
-  __shared__ uint32_t tmem_slot;
+  __shared__ __align__(8) unsigned long long bars[WARPS * FEW_SLOTS], halves[2];
   constexpr bool TENSOR = sizeof(T) == 2;
-  if (!TENSOR) pdl_launch();
+  pdl_launch();
+  if (TENSOR && threadIdx.x == 0) {
+    prefetch_map(&maps.x);
+    prefetch_map(&maps.whole);
+  }
   pdl_wait();
   const int tile = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;  // (of the list: part of a tile)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
@@ -500,7 +551,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
     const int* entry = p.tiles + tile / (LIST / TILE) * 3;
     const int first = tile % (LIST / TILE) * TILE;
     s = entry[0], count = min(TILE, entry[2] - first);
-    if (count > 0 && threadIdx.x < count) rows[threadIdx.x] = p.rows[entry[1] + first + threadIdx.x];
+    if (count > 0 && threadIdx.x < TILE) rows[threadIdx.x] = p.rows[entry[1] + first + min((int)threadIdx.x, count - 1)];  // (rows past the last: what comes of them is not read)
   } else {
     count = own_rows(p, tile, rows, s);
   }
@@ -517,28 +568,16 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
   const T* b = reinterpret_cast<const T*>(p.b) + (long long)s * p.N * p.R;
   // whole sections at a time, as many as there is room for
   const int together = min(p.sections, p.most / R16);
-  Tensor tn;
-  if constexpr (TENSOR) {
-    tn = make_tensor(p, smem, bars, &tmem_slot);  // (a barrier: the rows are there)
-    pdl_launch();                                 // not before it has its tensor memory: a kernel that waits for this one could hold it
-    if (threadIdx.x >= count && threadIdx.x < TILE) rows[threadIdx.x] = rows[0];  // (any row: what comes of it is not read)
+  if (threadIdx.x < WARPS * FEW_SLOTS + 2) {
+    tc::bar_init(threadIdx.x < 2 ? sm32(halves + threadIdx.x) : sm32(bars + threadIdx.x - 2), threadIdx.x < 2 ? WARPS : 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  // this CTA's eighth of B and of the rows that are added to comes on its way
-  const int per = (p.N / 8 + CLUSTER - 1) / CLUSTER * 8, c0 = rank * per, c1 = min(p.N, c0 + per);
-  if (c0 < c1) {
-    const char* from = reinterpret_cast<const char*>(b + (long long)c0 * p.R);
-    const int bytes = (c1 - c0) * p.R * (int)sizeof(T);
-    for (int i = threadIdx.x * 128; i < bytes; i += THREADS * 128) prefetch(from + i);
-    const int row = threadIdx.x / (THREADS / TILE), row_bytes = (c1 - c0) * (int)sizeof(O);
-    if (row < count) {
-      const char* at = reinterpret_cast<const char*>(reinterpret_cast<const O*>(p.base) + rows[row] * p.base_stride + c0);
-      for (int i = threadIdx.x % (THREADS / TILE) * 128; i < row_bytes; i += 128 * (THREADS / TILE)) prefetch(at + i);
-    }
-  }
   float* part = smem;                       // float32: [WARPS][TILE][PART]
-  float* sums = TENSOR ? reinterpret_cast<float*>(reinterpret_cast<char*>(smem) + p.slots * slot_bytes(TILE, p.most)) : smem + WARPS * TILE * PART;
-  T* inner = TENSOR ? reinterpret_cast<T*>(sums + CLUSTER * p.most * SUM_ROW) : reinterpret_cast<T*>(smem);
+  float* sums = reinterpret_cast<float*>(reinterpret_cast<char*>(smem) + p.stage);
+  T* inner = reinterpret_cast<T*>(sums + CLUSTER * TILE * p.most);
+  const int warp_floats = p.slots * slot_bytes(TILE, p.most) / 4;  // from a warp's slots to the next warp's
+  Few few{sm32(smem + warp * warp_floats), sm32(bars + warp * FEW_SLOTS), 0};
   Rows x;
   if constexpr (!TENSOR) {
     const char* from = reinterpret_cast<const char*>(p.x);
@@ -546,82 +585,122 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
     x.hi = g + 8 < count ? from + rows[g + 8] * p.x_stride * (long long)sizeof(T) : nullptr;
   }
   const float scale = p.scales[s];
-  const O* base0 = g < count ? reinterpret_cast<const O*>(p.base) + rows[g] * p.base_stride : nullptr;
-  const O* base1 = g + 8 < count ? reinterpret_cast<const O*>(p.base) + rows[g + 8] * p.base_stride : nullptr;
-  O* out0 = g < count ? reinterpret_cast<O*>(p.out) + rows[g] * p.out_stride : nullptr;
-  O* out1 = g + 8 < count ? reinterpret_cast<O*>(p.out) + rows[g + 8] * p.out_stride : nullptr;
+  // groups of 32 columns, in pieces whose columns of B and of the rows take half the stage each
+  const int half_bytes = p.stage / 2;
+  int pieces = 0;  // so far: what phase the halves' barriers are in
   for (int sec0 = 0; sec0 < p.sections; sec0 += together) {
     const int sec1 = min(p.sections, sec0 + together), total = (sec1 - sec0) * R16;
-    if constexpr (TENSOR) {
-      first_product<TILE>(p, maps, (s * p.sections + sec0) * p.R, rows, 0, total, R16, rank, tn, sums);
-    } else {
-      for (int t0 = 0; t0 < total; t0 += CHUNK) {
+    for (int t0 = 0; t0 < total; t0 += TENSOR ? MOST : CHUNK) {
+      // the warps' partial sums of `wide` numbers, `step` floats from one row to the next
+      const int wide = TENSOR ? total : min(CHUNK, total - t0), step = TENSOR ? total + 4 : PART, from = TENSOR ? warp_floats : TILE * PART;
+      if constexpr (TENSOR) {
+        first_product(p, maps, (s * p.sections + sec0) * p.R, rows, total, R16, rank, few, smem + warp * warp_floats);
+      } else {
         first_product(p, a + (long long)sec0 * p.R * p.K, x, t0, total, R16, rank * WARPS + warp, part + warp * TILE * PART);
-        // the CTAs of the cluster run, and have read the sums of the sections before: their memory may be written
-        if (t0 == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        __syncthreads();
-        const int wide = min(CHUNK, total - t0);
-        const int row = threadIdx.x / (THREADS / TILE), t = threadIdx.x % (THREADS / TILE) * 4;
-        static_assert(CHUNK / 4 <= THREADS / TILE, "sixteen threads a row take four numbers each");
-        if (t < wide) {
-          float4 v = *reinterpret_cast<const float4*>(part + row * PART + t);
-#pragma unroll
-          for (int w = 1; w < WARPS; ++w) {
-            const float4 o = *reinterpret_cast<const float4*>(part + (w * TILE + row) * PART + t);
-            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-          }
-          const uint32_t to = sm32(sums + (rank * TILE + row) * total + t0 + t);
-#pragma unroll
-          for (int c = 0; c < CLUSTER; ++c) st_cluster(to, c, v);
-        }
-        __syncthreads();
       }
+      // the CTAs of the cluster run, and have read the sums of the sections before: their memory may be written
+      if (t0 == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+      __syncthreads();
+      const int row = threadIdx.x / (THREADS / TILE);
+      for (int t = threadIdx.x % (THREADS / TILE) * 4; t < wide; t += THREADS / TILE * 4) {
+        float4 v = *reinterpret_cast<const float4*>(smem + row * step + t);
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) {
+          const float4 o = *reinterpret_cast<const float4*>(smem + w * from + row * step + t);
+          v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+        }
+        const uint32_t to = sm32(sums + (rank * TILE + row) * total + t0 + t);
+#pragma unroll
+        for (int c = 0; c < CLUSTER; ++c) st_cluster(to, c, v);
+      }
+      if (TENSOR) tc::fence_async_smem();  // (before the next sections' copies into the same place)
+      __syncthreads();
     }
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    // groups of 32 columns of one section, a warp each; the first ones are fetched while the cluster meets
-    const int before = sec0 ? p.groups[sec0 - 1] : 0, groups = p.groups[sec1 - 1] - before, mine = (groups + CLUSTER - 1) / CLUSTER;
-    const auto group = [&](Group<T, O>& gr, int i) {
-      const int gi = rank * mine + i;
-      gr.gi = i < mine && gi < groups ? gi + before : -1;
-      fetch(gr, p, b, base0, base1);
+    // (alternating sections lie side by side: their groups are taken together, or, one section at a time, with what lies between them)
+    const bool both = p.alternating && sec1 - sec0 == 2, one = p.alternating && !both;
+    const int all_groups = both ? 2 * ((p.width[0] + 31) / 32) : one ? (p.width[0] + 31) / 32 : p.groups[sec1 - 1] - (sec0 ? p.groups[sec0 - 1] : 0);
+    const int pair = both ? 2 : 1, mine = ((all_groups + CLUSTER - 1) / CLUSTER + pair - 1) / pair * pair;
+    const int begin = rank * mine, end = min(all_groups, begin + mine);
+    const auto locate = [&](int gi, int& i) {  // section and number there of this pass's group gi
+      if (one) {
+        i = gi;
+        return Section{sec0, 0, p.width[0]};
+      }
+      if (!p.alternating && sec0) gi += p.groups[sec0 - 1];
+      const Section sc = section_of_group(p, gi);
+      i = gi;
+      return sc;
     };
-    Group<T, O> ahead[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) group(ahead[i], warp + i * WARPS);
+    const int span = (one ? 64 : 32) * (p.R * (int)sizeof(T) + TILE * (int)sizeof(O));
+    const int each = max(pair, (half_bytes - TILE * 128) / span / pair * pair);  // groups of a piece
+    const auto columns = [&](int g0, int& c0, int& c1) {  // of the piece that begins with group g0
+      const int last = min(end, g0 + each) - 1;
+      int i;
+      const Section s0 = locate(g0, i);
+      c0 = p.alternating ? i * 64 : s0.begin + 32 * i;
+      const Section s1 = locate(last, i);
+      c1 = p.alternating ? min(p.N, i * 64 + 64) : s1.begin + min(s1.width, 32 * i + 32);
+    };
+    const auto row_stride = [&](int c0, int c1) { return ((c1 - c0) * (int)sizeof(O) + 63) / 128 * 128 + 64; };  // (two rows in all banks)
+    const auto load = [&](int g0, int half) {  // a thread of every warp
+      int c0, c1;
+      columns(g0, c0, c1);
+      const uint32_t bar = sm32(halves + half), at = sm32(smem) + half * half_bytes;
+      const uint32_t b_bytes = (c1 - c0) * p.R * sizeof(T), r_bytes = (c1 - c0) * sizeof(O);
+      const int r1 = warp + WARPS < count;
+      tc::bar_expect_tx(bar, (warp == 0 ? b_bytes : 0) + (warp < count ? r_bytes : 0) + (r1 ? r_bytes : 0));
+      if (warp == 0) bulk_load(at, b + (long long)c0 * p.R, b_bytes, bar);
+      for (int r = warp; r < count; r += WARPS)
+        bulk_load(at + b_bytes + r * row_stride(c0, c1), reinterpret_cast<const O*>(p.base) + rows[r] * p.base_stride + c0, r_bytes, bar);
+    };
+    if (begin < end && elect_one()) load(begin, pieces & 1);
+    __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if constexpr (TENSOR) {
-      for (int i = threadIdx.x; i < TILE * total; i += THREADS) {
-        const int row = i % TILE, t = i / TILE;
-        float v = 0.f;
+    for (int row = threadIdx.x / (THREADS / TILE), t = threadIdx.x % (THREADS / TILE); t < total; t += THREADS / TILE) {
+      float v = 0.f;
 #pragma unroll
-        for (int c = 0; c < CLUSTER; ++c) v += sums[(c * total + t) * SUM_ROW + row];
-        keep_inner<SPLITS>(inner, total, row, t, v * scale);
-      }
-    } else {
-      for (int row = threadIdx.x / (THREADS / TILE), t = threadIdx.x % (THREADS / TILE); t < total; t += THREADS / TILE) {
-        float v = 0.f;
-#pragma unroll
-        for (int c = 0; c < CLUSTER; ++c) v += sums[(c * TILE + row) * total + t];
-        keep_inner<SPLITS>(inner, total, row, t, v * scale);
-      }
+      for (int c = 0; c < CLUSTER; ++c) v += sums[(c * TILE + row) * total + t];
+      keep_inner<SPLITS>(inner, total, row, t, v * scale);
     }
     __syncthreads();
     if (sec1 < p.sections) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    for (int i = warp; i < mine; i += AHEAD * WARPS) {
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        const Group<T, O> gr = ahead[j];
-        if (gr.gi < 0) continue;
-        group(ahead[j], i + (j + AHEAD) * WARPS);
+    for (int g0 = begin; g0 < end; g0 += each, ++pieces) {
+      const int half = pieces & 1;
+      // (the other half has been read: a barrier lies behind its piece)
+      if (g0 + each < end && elect_one()) load(g0 + each, half ^ 1);
+      __syncwarp();
+      tc::bar_wait(sm32(halves + half), pieces >> 1 & 1, p.err);
+      int c0, c1;
+      columns(g0, c0, c1);
+      const char* at = reinterpret_cast<const char*>(smem) + half * half_bytes;
+      const T* bs = reinterpret_cast<const T*>(at);
+      const char* base = at + (c1 - c0) * p.R * sizeof(T);
+      const int stride = row_stride(c0, c1);
+      for (int gi = g0 + warp; gi < min(end, g0 + each); gi += WARPS) {
+        int i;
+        const Section sc = locate(gi, i);
         float acc[2][8];
-        second_product<SPLITS>(p, b, inner, total, sec0, gr, R16, acc);
-        if (gr.col >= 0 && out0) add_eight(gr.base[0], out0 + gr.col, acc[0]);
-        if (gr.col >= 0 && out1) add_eight(gr.base[1], out1 + gr.col, acc[1]);
+        second_product<SPLITS>(p, bs, c0, inner + (sc.sec - sec0) * R16, total, sc, i * 32, R16, acc);
+        const int u = i * 32 + 8 * (lane & 3);
+        if (u < sc.width) {
+          const int c = column(p, sc, u);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = g + 8 * h;
+            if (r < count) {
+              uint4 old[sizeof(O) / 2];
+#pragma unroll
+              for (int k = 0; k < (int)sizeof(O) / 2; ++k) old[k] = reinterpret_cast<const uint4*>(base + r * stride + (c - c0) * sizeof(O))[k];
+              add_eight(old, reinterpret_cast<O*>(p.out) + rows[r] * p.out_stride + c, acc[h]);
+            }
+          }
+        }
       }
+      tc::fence_async_smem();  // what was read here comes before what is copied here next
+      __syncthreads();
     }
-    __syncthreads();
   }
-  if constexpr (TENSOR) free_tensor(p, tn);
 }
 
 // ---- many rows, first kernel: the inner numbers of 128 rows by a cluster, of which CTA c keeps rows 16c .. 16c + 15
@@ -632,6 +711,10 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) adapt
   __shared__ unsigned runs_of[LIST / 32];
   __shared__ __align__(8) unsigned long long bars[BARS];
   __shared__ uint32_t tmem_slot;
+  if (threadIdx.x == 0) {
+    prefetch_map(&maps.run);
+    prefetch_map(&maps.whole);
+  }
   pdl_wait();
   const int tile = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;
   const int s = p.tiles[3 * tile], first = p.tiles[3 * tile + 1], count = p.tiles[3 * tile + 2];
@@ -654,7 +737,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) adapt
   const int wide = p.sections * p.R;  // numbers of a row of `inner`
   for (int sec0 = 0; sec0 < p.sections; sec0 += together) {
     const int sec1 = min(p.sections, sec0 + together), total = (sec1 - sec0) * R16;
-    first_product<LIST>(p, maps, (s * p.sections + sec0) * p.R, rows, runs, total, R16, rank, tn, sums);
+    first_product(p, maps, (s * p.sections + sec0) * p.R, rows, runs, total, R16, rank, tn, sums);
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     // two neighbouring numbers of a row a thread
     bf16* inner = p.inner + ((long long)tile * SPLITS * LIST + rank * TILE) * wide + sec0 * R16;
@@ -806,19 +889,40 @@ __global__ void __launch_bounds__(THREADS, 2) adapter_outer_kernel(const __grid_
   }
 }
 
-// How many blocks of k shared memory holds, the columns of tensor memory; the bytes for the ring, the sums and the inner numbers (and 16 KB: the
-// last lanes of the accumulator read past the rows of A).
-size_t ring_smem(AdapterParams& p, int nr, int splits, size_t budget) {
-  const size_t rest = (size_t)CLUSTER * p.most * SUM_ROW * 4 + (nr == TILE ? (size_t)splits * TILE * (p.most + 16) * 2 : 0) + 16 * 1024, slot = slot_bytes(nr, p.most);
-  const int blocks = ((p.K + BLOCK_K - 1) / BLOCK_K + CLUSTER - 1) / CLUSTER;
-  p.slots = (int)(budget > rest ? (budget - rest) / slot : 0);
-  p.slots = max(1, min(min(p.slots, MAX_SLOTS), blocks));
-  p.tmem = 32;
-  while (p.tmem < (p.most + 127) / 128 * nr) p.tmem *= 2;
-  return p.slots * slot + rest;
+// Few rows: slots a warp (one where it has one block, or where two keep a second CTA off the SM), the stage, and the bytes for it, the sums and
+// the inner numbers.
+template <typename T, typename O>
+size_t few_smem(AdapterParams& p, int splits) {
+  const size_t rest = (size_t)CLUSTER * TILE * p.most * 4 + (sizeof(T) == 2 ? (size_t)splits * TILE * (p.most + 16) * 2 : (size_t)TILE * (p.most + 4) * 4);
+  p.slots = 1;
+  size_t stage = 64 * 1024;
+  if (sizeof(T) == 2) {
+    const int blocks = ((p.K + BLOCK_K - 1) / BLOCK_K + CLUSTER - 1) / CLUSTER;
+    const size_t slots = (size_t)WARPS * slot_bytes(TILE, p.most);
+    if (blocks > WARPS && rest + 2 * slots <= 112 * 1024) p.slots = FEW_SLOTS;
+    stage = max(p.slots * slots, min(stage, (size_t)(112 * 1024 - min(rest, (size_t)48 * 1024))));
+  }
+  // two groups at least (or one, and what lies between its columns) in each half
+  stage = max(stage, (size_t)2 * (64 * (p.R * sizeof(T) + TILE * sizeof(O)) + TILE * 256));
+  p.stage = (int)((stage + 2047) / 2048 * 2048);
+  return rest + p.stage;
 }
 
-// x: [n][K], one row a box and 32; A: [S sections R][K], sixteen rows a box; zeros past K
+// Many rows: blocks of k that shared memory holds, columns of tensor memory, and the bytes for the ring and the sums (and 16 KB: the last lanes of
+// the accumulator read past the rows of A).
+size_t many_smem(AdapterParams& p) {
+  const size_t rest = (size_t)CLUSTER * p.most * SUM_ROW * 4 + 16 * 1024, slot = slot_bytes(LIST, p.most), budget = 220 * 1024;
+  const int blocks = ((p.K + BLOCK_K - 1) / BLOCK_K + CLUSTER - 1) / CLUSTER;
+  p.slots = max(1, min(min((int)((budget - rest) / slot), MAX_SLOTS), blocks));
+  p.tmem = LIST;
+  return p.slots * slot + rest;
+}
+static_assert(MOST <= 128 && CLUSTER * MOST * SUM_ROW * 4 + 16 * 1024 + slot_bytes(LIST, MOST) <= 220 * 1024, "one tile of the accumulator; room for a block");
+static_assert(CLUSTER * TILE * MOST * 4 + 3 * TILE * (MOST + 16) * 2 + WARPS * slot_bytes(TILE, MOST) <= 226 * 1024, "room for a block a warp");
+static_assert(CLUSTER * TILE * MOST * 4 + TILE * (MOST + 4) * 4 + 2 * (64 * (MOST * 4 + TILE * 4) + TILE * 256) + 2048 <= 226 * 1024, "... and for a float32 group a half");
+static_assert(TILE * (MOST + 4) * 4 <= slot_bytes(TILE, MOST) && TILE * (16 + 4) * 4 <= slot_bytes(TILE, 16), "partial sums take a slot's place");
+
+// x: [n][K], one row a box and 32; A: [S sections R][K], sixteen rows a box and `most`; zeros past K
 int make_maps(const AdapterParams& p, Maps& maps) {
   tc::EncodeTiledFn fn = tc::encode_tiled();
   if (!fn) return (int)cudaErrorNotSupported;
@@ -829,13 +933,15 @@ int make_maps(const AdapterParams& p, Maps& maps) {
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(at), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
-  return encode(&maps.x, p.x, p.n, p.x_stride, 1) && encode(&maps.run, p.x, p.n, p.x_stride, 32) && encode(&maps.a, p.a, (long long)p.S * p.sections * p.R, p.K, 16) ? 0 : (int)cudaErrorInvalidValue;
+  return encode(&maps.x, p.x, p.n, p.x_stride, 1) && encode(&maps.run, p.x, p.n, p.x_stride, 32) && encode(&maps.a, p.a, (long long)p.S * p.sections * p.R, p.K, 16) &&
+                 encode(&maps.whole, p.a, (long long)p.S * p.sections * p.R, p.K, p.most)
+             ? 0 : (int)cudaErrorInvalidValue;
 }
 
 template <typename O, int SPLITS>
 int run_wide(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
   const int total = p.sections * p.R, groups = p.groups[MAX_SECTIONS - 1];
-  const size_t one = ring_smem(p, LIST, SPLITS, 220 * 1024), two = (size_t)SPLITS * ROWS * inner_stride(total, 2) * 2;
+  const size_t one = many_smem(p), two = (size_t)SPLITS * ROWS * inner_stride(total, 2) * 2;
   const auto inner = adapter_inner_kernel<SPLITS>;
   const auto outer = adapter_outer_kernel<O, SPLITS>;
   cudaError_t rc = cudaFuncSetAttribute(inner, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one);
@@ -933,8 +1039,8 @@ __global__ void __launch_bounds__(SORT) adapter_group_kernel(const int* __restri
 
 template <typename T, typename O, int SPLITS>
 int run_tiles(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
-  static_assert(TILE * (MOST + 4) * 4 <= WARPS * TILE * PART * 4, "the inner numbers take the partial sums' place");
-  const size_t smem = sizeof(T) == 2 ? ring_smem(p, TILE, SPLITS, 112 * 1024) : (size_t)(WARPS * TILE * PART + CLUSTER * TILE * p.most) * 4;
+  static_assert(WARPS * TILE * PART * 4 <= 64 * 1024, "the partial sums take the stage's place");
+  const size_t smem = few_smem<T, O>(p, SPLITS);
   const auto kernel = adapter_tile_kernel<T, O, SPLITS>;
   const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (rc != cudaSuccess) return (int)rc;
@@ -990,7 +1096,7 @@ int run(AdapterParams& p, const int* ends, int wide, int max_tiles, int two, cud
   KVF_API int kvf_adapter_add_##SUF(const void* x, long long x_stride, const void* a, const void* b, const float* scales, const int* ranks, const int* ids, int n, int S,  \
                                     int sections, int R, int K, int N, int end0, int end1, int end2, int alternating, const void* base, long long base_stride, void* out,  \
                                     long long out_stride, int wide, const int* rows, const int* tiles, int max_tiles, void* inner, int two, int* err, cudaStream_t st) {   \
-    AdapterParams p{x, a, b, scales, ranks, ids, rows, tiles, (bf16*)inner, base, out, err, x_stride, base_stride, out_stride, n, S, sections, R, K, N, {}, {}, {}, alternating, 0, 0, 0}; \
+    AdapterParams p{x, a, b, scales, ranks, ids, rows, tiles, (bf16*)inner, base, out, err, x_stride, base_stride, out_stride, n, S, sections, R, K, N, {}, {}, {}, alternating, 0, 0, 0, 0}; \
     const int ends[3] = {end0, end1, end2};                                                                                                                               \
     return run<T, WIDE_SPLITS>(p, ends, wide, max_tiles, two, st);                                                                                                             \
   }
