@@ -394,19 +394,18 @@ __device__ __forceinline__ void keep_inner(float* inner, int total, int row, int
   inner[row * inner_stride(total, 4) + t] = v;
 }
 
-// A group of 32 columns of a section: its own 16 numbers a row of B ... in shared memory (`b`, from column `c0` on) and the inner numbers make
-// acc[row half][column], eight columns a lane.
+// Of a group of columns (32, or 64 where the sections alternate) the 32 of one section: rows of B in shared memory (`b`, the group's first column's,
+// `last` what is there after it) and the section's inner numbers make acc[row half][column], eight columns a lane: 8q .. 8q + 7 of the 32.
 // Column 2q + e of the j-th of four tensor-core tiles is column 8q + 2j + e of the 32, so that a lane's eight results lie side by side.
+__device__ __forceinline__ int in_group(const AdapterParams& p, int sec, int u) { return p.alternating ? (u >> 3) * 16 + sec * 8 + (u & 7) : u; }
+
 template <int SPLITS>
-__device__ __forceinline__ void second_product(const AdapterParams& p, const bf16* b, int c0, const bf16* inner, int total, const Section& s, int u0, int R16, float (&acc)[2][8]) {
+__device__ __forceinline__ void second_product(const AdapterParams& p, const bf16* b, int last, const bf16* inner, int total, int sec, int R16, float (&acc)[2][8]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int stride = inner_stride(total, 2);
   const bf16* rows[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int u = min(u0 + (g >> 1) * 8 + 2 * j + (g & 1), s.width - 1);  // (columns past the section's are not written)
-    rows[j] = b + (column(p, s, u) - c0) * p.R + 4 * q;
-  }
+  for (int j = 0; j < 4; ++j) rows[j] = b + min(in_group(p, sec, (g >> 1) * 8 + 2 * j + (g & 1)), last) * p.R + 4 * q;  // (columns past the last are not written)
   float c[4][4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -433,13 +432,14 @@ __device__ __forceinline__ void second_product(const AdapterParams& p, const bf1
 }
 
 template <int SPLITS>
-__device__ __forceinline__ void second_product(const AdapterParams& p, const float* b, int c0, const float* inner, int total, const Section& s, int u0, int R16, float (&acc)[2][8]) {
+__device__ __forceinline__ void second_product(const AdapterParams& p, const float* b, int last, const float* inner, int total, int sec, int R16, float (&acc)[2][8]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int stride = inner_stride(total, 4);
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[0][i] = acc[1][i] = 0.f;
-  if (u0 + 8 * q >= s.width) return;
-  const float* rows = b + (column(p, s, u0 + 8 * q) - c0) * p.R;
+  const int first = in_group(p, sec, 8 * q);
+  if (first > last) return;
+  const float* rows = b + first * p.R;
   const float* lo = inner + g * stride;
   const float* hi = lo + 8 * stride;
   for (int r = 0; r < R16; r += 4) {
@@ -617,42 +617,27 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
       __syncthreads();
     }
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    // (alternating sections lie side by side: their groups are taken together, or, one section at a time, with what lies between them)
-    const bool both = p.alternating && sec1 - sec0 == 2, one = p.alternating && !both;
-    const int all_groups = both ? 2 * ((p.width[0] + 31) / 32) : one ? (p.width[0] + 31) / 32 : p.groups[sec1 - 1] - (sec0 ? p.groups[sec0 - 1] : 0);
-    const int pair = both ? 2 : 1, mine = ((all_groups + CLUSTER - 1) / CLUSTER + pair - 1) / pair * pair;
-    const int begin = rank * mine, end = min(all_groups, begin + mine);
-    const auto locate = [&](int gi, int& i) {  // section and number there of this pass's group gi
-      if (one) {
-        i = gi;
-        return Section{sec0, 0, p.width[0]};
+    // the sections' columns lie side by side (alternating ones among each other), from `left` to `right`, in groups of `group` columns
+    int left = 0, right = p.N;
+    if (!p.alternating) {
+#pragma unroll
+      for (int i = 1; i < MAX_SECTIONS; ++i) {
+        if (sec0 == i) left = p.begin[i];
+        if (sec1 == i) right = p.begin[i];
       }
-      if (!p.alternating && sec0) gi += p.groups[sec0 - 1];
-      const Section sc = section_of_group(p, gi);
-      i = gi;
-      return sc;
-    };
-    const int span = (one ? 64 : 32) * (p.R * (int)sizeof(T) + TILE * (int)sizeof(O));
-    const int each = max(pair, (half_bytes - TILE * 128) / span / pair * pair);  // groups of a piece
-    const auto columns = [&](int g0, int& c0, int& c1) {  // of the piece that begins with group g0
-      const int last = min(end, g0 + each) - 1;
-      int i;
-      const Section s0 = locate(g0, i);
-      c0 = p.alternating ? i * 64 : s0.begin + 32 * i;
-      const Section s1 = locate(last, i);
-      c1 = p.alternating ? min(p.N, i * 64 + 64) : s1.begin + min(s1.width, 32 * i + 32);
-    };
-    const auto row_stride = [&](int c0, int c1) { return ((c1 - c0) * (int)sizeof(O) + 63) / 128 * 128 + 64; };  // (two rows in all banks)
+    }
+    const int group = p.alternating ? 64 : 32, groups = (right - left + group - 1) / group, mine = (groups + CLUSTER - 1) / CLUSTER;
+    const int begin = rank * mine, end = min(groups, begin + mine);
+    const int each = max(1, (half_bytes - TILE * 128) / (group * (p.R * (int)sizeof(T) + TILE * (int)sizeof(O))));  // groups of a piece
+    const auto row_stride = [&](int columns) { return (columns * (int)sizeof(O) + 63) / 128 * 128 + 64; };  // (two rows in all banks)
     const auto load = [&](int g0, int half) {  // a thread of every warp
-      int c0, c1;
-      columns(g0, c0, c1);
+      const int c0 = left + g0 * group, columns = min(right, left + min(end, g0 + each) * group) - c0;
       const uint32_t bar = sm32(halves + half), at = sm32(smem) + half * half_bytes;
-      const uint32_t b_bytes = (c1 - c0) * p.R * sizeof(T), r_bytes = (c1 - c0) * sizeof(O);
-      const int r1 = warp + WARPS < count;
-      tc::bar_expect_tx(bar, (warp == 0 ? b_bytes : 0) + (warp < count ? r_bytes : 0) + (r1 ? r_bytes : 0));
+      const uint32_t b_bytes = columns * p.R * sizeof(T), r_bytes = columns * sizeof(O);
+      tc::bar_expect_tx(bar, (warp == 0 ? b_bytes : 0) + (warp < count ? r_bytes : 0) + (warp + WARPS < count ? r_bytes : 0));
       if (warp == 0) bulk_load(at, b + (long long)c0 * p.R, b_bytes, bar);
       for (int r = warp; r < count; r += WARPS)
-        bulk_load(at + b_bytes + r * row_stride(c0, c1), reinterpret_cast<const O*>(p.base) + rows[r] * p.base_stride + c0, r_bytes, bar);
+        bulk_load(at + b_bytes + r * row_stride(columns), reinterpret_cast<const O*>(p.base) + rows[r] * p.base_stride + c0, r_bytes, bar);
     };
     if (begin < end && elect_one()) load(begin, pieces & 1);
     __syncwarp();
@@ -671,28 +656,27 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
       if (g0 + each < end && elect_one()) load(g0 + each, half ^ 1);
       __syncwarp();
       tc::bar_wait(sm32(halves + half), pieces >> 1 & 1, p.err);
-      int c0, c1;
-      columns(g0, c0, c1);
+      const int c0 = left + g0 * group, columns = min(right, left + min(end, g0 + each) * group) - c0, stride = row_stride(columns);
       const char* at = reinterpret_cast<const char*>(smem) + half * half_bytes;
-      const T* bs = reinterpret_cast<const T*>(at);
-      const char* base = at + (c1 - c0) * p.R * sizeof(T);
-      const int stride = row_stride(c0, c1);
+      const char* base = at + columns * p.R * sizeof(T);
       for (int gi = g0 + warp; gi < min(end, g0 + each); gi += WARPS) {
-        int i;
-        const Section sc = locate(gi, i);
-        float acc[2][8];
-        second_product<SPLITS>(p, bs, c0, inner + (sc.sec - sec0) * R16, total, sc, i * 32, R16, acc);
-        const int u = i * 32 + 8 * (lane & 3);
-        if (u < sc.width) {
-          const int c = column(p, sc, u);
+        const int from = (gi - g0) * group;  // the group's first column, from the piece's
+#pragma unroll
+        for (int i = 0; i < MAX_SECTIONS; ++i) {
+          // (a group may reach over the end of a section: each takes its own columns)
+          if (i < sec0 || i >= sec1 || (!p.alternating && (c0 + from >= p.begin[i] + p.width[i] || c0 + from + 32 <= p.begin[i]))) continue;
+          float acc[2][8];
+          second_product<SPLITS>(p, reinterpret_cast<const T*>(at) + from * p.R, columns - 1 - from, inner + (i - sec0) * R16, total, i, R16, acc);
+          const int c = from + in_group(p, i, 8 * (lane & 3));
+          if (c >= columns || (!p.alternating && (c0 + c < p.begin[i] || c0 + c >= p.begin[i] + p.width[i]))) continue;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int r = g + 8 * h;
             if (r < count) {
               uint4 old[sizeof(O) / 2];
 #pragma unroll
-              for (int k = 0; k < (int)sizeof(O) / 2; ++k) old[k] = reinterpret_cast<const uint4*>(base + r * stride + (c - c0) * sizeof(O))[k];
-              add_eight(old, reinterpret_cast<O*>(p.out) + rows[r] * p.out_stride + c, acc[h]);
+              for (int k = 0; k < (int)sizeof(O) / 2; ++k) old[k] = reinterpret_cast<const uint4*>(base + r * stride + c * sizeof(O))[k];
+              add_eight(old, reinterpret_cast<O*>(p.out) + rows[r] * p.out_stride + c0 + c, acc[h]);
             }
           }
         }
