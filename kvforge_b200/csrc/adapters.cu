@@ -49,36 +49,13 @@ struct AdapterParams {
   int* err;
   long long x_stride, base_stride, out_stride;
   int n, S, sections, R, K, N;
-  // sections: where they begin, how wide they are, and the groups of 32 columns up to their end
-  int begin[MAX_SECTIONS], width[MAX_SECTIONS], groups[MAX_SECTIONS];
+  int begin[MAX_SECTIONS], width[MAX_SECTIONS];  // of the sections
   int alternating;
   int most;   // inner numbers of a row that shared memory holds at a time (whole sections of rank R)
   int stage;  // bytes of shared memory that columns of B and of the rows take in turn (few rows)
   int slots;  // blocks of 64 columns of k that it holds (of a warp, where there are few rows; bf16)
   int tmem;   // columns of tensor memory
 };
-
-// A section as a lane needs it (taken from the parameters with fixed indices: an index known only at run time costs a constant load's
-// latency each time).
-struct Section {
-  int sec, begin, width;
-};
-// The section of group `gi` of 32 columns; gi becomes its number there.  Alternating sections take turns, so that groups that follow one another
-// lie side by side.
-__device__ __forceinline__ Section section_of_group(const AdapterParams& p, int& gi) {
-  Section s{0, p.begin[0], p.width[0]};
-  if (p.alternating) {
-    s.sec = gi & 1;
-    gi >>= 1;
-    return s;
-  }
-  int before = 0;
-#pragma unroll
-  for (int i = 1; i < MAX_SECTIONS; ++i)
-    if (gi >= p.groups[i - 1]) s = Section{i, p.begin[i], p.width[i]}, before = p.groups[i - 1];
-  gi -= before;
-  return s;
-}
 
 __device__ __forceinline__ uint32_t sm32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -109,9 +86,6 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
                : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const void* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory"); }
-
-// Column of the result that is number u of a section.
-__device__ __forceinline__ int column(const AdapterParams& p, const Section& s, int u) { return p.alternating ? (u >> 3) * 16 + s.sec * 8 + (u & 7) : s.begin + u; }
 
 // ---- the first product in float32: partial sums over a warp's share of k for 16 rows and CHUNK rows of A, into part[16][PART]
 // k goes in steps of 32, eight a lane; step st belongs to warp st % 64 of the cluster
@@ -277,10 +251,12 @@ __device__ __forceinline__ void first_product(const AdapterParams& p, const Maps
   if (warp > 0) {
     // Warp w fills slot w - 1 and no other, one block after another: what it waits for is never more than one phase ahead of the barrier
     // (a parity tells only two neighbouring phases apart).
-    if (warp <= p.slots && elect_one()) {
-      const int slot = warp - 1, begin = tn.block % p.slots;
-      for (int j = slot - begin + (slot < begin ? p.slots : 0); j < blocks; j += p.slots) {
-        const int turn = (tn.block + j) / p.slots;
+    // Where all rows follow one another a block is a few copies, and one warp starts them block after block: the first block is there first.
+    const bool alone = runs == (1u << LIST / 32) - 1;
+    if (warp <= (alone ? 1 : p.slots) && elect_one()) {
+      const int begin = tn.block % p.slots, own = warp - 1;
+      for (int j = alone ? 0 : own - begin + (own < begin ? p.slots : 0); j < blocks; j += alone ? 1 : p.slots) {
+        const int turn = (tn.block + j) / p.slots, slot = (tn.block + j) % p.slots;
         if (turn) tc::bar_wait(done + 8 * slot, (turn - 1) & 1, p.err);
         const uint32_t to = tn.ring + slot * bytes, bar = filled + 8 * slot;
         tc::bar_expect_tx(bar, bytes);
@@ -451,12 +427,6 @@ __device__ __forceinline__ void second_product(const AdapterParams& p, const flo
       acc[1][i] = fmaf(w.w, h.w, fmaf(w.z, h.z, fmaf(w.y, h.y, fmaf(w.x, h.x, acc[1][i]))));
     }
   }
-}
-
-// Row of B (in memory) for the lane's column of the j-th tensor-core tile.
-__device__ __forceinline__ const bf16* b_row(const AdapterParams& p, const bf16* b, const Section& s, int u0, int j) {
-  const int g = (threadIdx.x & 31) >> 2, u = u0 + (g >> 1) * 8 + 2 * j + (g & 1);
-  return u < s.width ? b + (long long)column(p, s, u) * p.R : nullptr;
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -668,17 +638,18 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
           float acc[2][8];
           second_product<SPLITS>(p, reinterpret_cast<const T*>(at) + from * p.R, columns - 1 - from, inner + (i - sec0) * R16, total, i, R16, acc);
           const int c = from + in_group(p, i, 8 * (lane & 3));
-          if (c >= columns || (!p.alternating && (c0 + c < p.begin[i] || c0 + c >= p.begin[i] + p.width[i]))) continue;
+          const bool own = c < columns && (p.alternating || (c0 + c >= p.begin[i] && c0 + c < p.begin[i] + p.width[i]));
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int r = g + 8 * h;
-            if (r < count) {
+            if (own && r < count) {
               uint4 old[sizeof(O) / 2];
 #pragma unroll
               for (int k = 0; k < (int)sizeof(O) / 2; ++k) old[k] = reinterpret_cast<const uint4*>(base + r * stride + c * sizeof(O))[k];
               add_eight(old, reinterpret_cast<O*>(p.out) + rows[r] * p.out_stride + c0 + c, acc[h]);
             }
           }
+          __syncwarp();  // (the next products take the whole warp)
         }
       }
       tc::fence_async_smem();  // what was read here comes before what is copied here next
@@ -751,125 +722,245 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) adapt
   free_tensor(p, tn);
 }
 
-// ---- many rows, second kernel: ROWS rows and `each` groups of 32 columns a warp, one after another; a group's pieces of the rows are fetched while
-// the group before is multiplied
-constexpr int ROWS = 64;
+// ---- many rows, second kernel: a tile's rows and a stripe of columns a CTA, 64 columns at a time.  A warp of its own fetches what the pieces need (the
+// rows by TMA, 32 that follow one another a box or four gathered; the columns' rows of B are one stretch), several pieces ahead; eight
+// warps multiply, add and write 16 rows and 32 columns at a time.  What is on its way is in shared memory, not in registers: with the
+// rows in registers, fetched a group ahead, 2,048 rows of 6144 columns took 43 us in all and 1.3 TB/s here.
+constexpr int PIECE = 64;  // columns
+constexpr int MAX_STAGES = 4;
+// eight rows of B and 64 bytes, so that the lanes of a load (rows two apart in pairs, eight apart) lie in different banks
+__host__ __device__ constexpr int b_block(int R) { return 8 * R * 2 + 64; }
+__host__ __device__ constexpr int b_stage(int R) { return (PIECE / 8 * b_block(R) + 1023) / 1024 * 1024; }  // (the next piece's swizzled rows begin at a multiple of 1,024)
 
-template <typename O, int SPLITS>
-__global__ void __launch_bounds__(THREADS, 2) adapter_outer_kernel(const __grid_constant__ AdapterParams p, int each) {
-  extern __shared__ __align__(16) bf16 held[];  // the rows' inner numbers: [SPLITS][ROWS][stride]
-  __shared__ int rows[ROWS];
+struct RowMaps {
+  CUtensorMap run, row;  // the rows that are added to, 128 bytes a box: 32 rows, one row
+};
+
+// KEPT: sixteens of inner numbers that stay in registers from piece to piece
+template <typename O, int SPLITS, int KEPT>
+__global__ void __launch_bounds__(THREADS + 32, KEPT > 1 ? 1 : 2) adapter_outer_kernel(const __grid_constant__ AdapterParams p, const __grid_constant__ RowMaps maps, int stripe, int stages) {
+  extern __shared__ __align__(1024) char ring[];  // a piece: [128 bytes' columns][LIST rows][128 bytes], then its rows of B
+  __shared__ int rows[LIST];
+  __shared__ unsigned runs[LIST / 32];
+  __shared__ __align__(8) unsigned long long filled[MAX_STAGES], empty[MAX_STAGES];
+  constexpr int ACROSS = PIECE * (int)sizeof(O) / 128;  // boxes of 128 bytes across a piece
+  constexpr int COLUMNS = 128 / (int)sizeof(O);
   pdl_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-  const int tile = blockIdx.y / (LIST / ROWS), r0 = blockIdx.y % (LIST / ROWS) * ROWS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, tile = blockIdx.y;
+  if (threadIdx.x < MAX_STAGES) {
+    tc::bar_init(sm32(filled + threadIdx.x), 1);
+    tc::bar_init(sm32(empty + threadIdx.x), WARPS);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == THREADS) {
+    prefetch_map(&maps.run);
+    prefetch_map(&maps.row);
+  }
   pdl_wait();
-  const int s = p.tiles[3 * tile], first = p.tiles[3 * tile + 1] + r0, count = min(ROWS, p.tiles[3 * tile + 2] - r0);
+  const int s = p.tiles[3 * tile], first = p.tiles[3 * tile + 1], count = p.tiles[3 * tile + 2];
   if (count <= 0) return;
-  if (threadIdx.x < ROWS) rows[threadIdx.x] = threadIdx.x < count ? p.rows[first + threadIdx.x] : -1;
+  if (threadIdx.x < LIST) {
+    const int row = p.rows[first + min((int)threadIdx.x, count - 1)];  // (rows past the last are fetched and not used)
+    const bool run = __all_sync(0xffffffffu, row == __shfl_sync(0xffffffffu, row, 0) + lane);
+    rows[threadIdx.x] = row;
+    if (lane == 0) runs[threadIdx.x / 32] = run;
+  }
   __syncthreads();
   const int R = s < 0 ? 0 : p.ranks ? min(max(p.ranks[s], 0), p.R) : p.R;
   if (R == 0) {
-    copy_rows<O>(p, rows, count, blockIdx.x, gridDim.x);
+    if (threadIdx.x < THREADS) copy_rows<O>(p, rows, count, blockIdx.x, gridDim.x);
     return;
   }
-  const int R16 = (R + 15) & ~15, total = p.sections * R16, wide = p.sections * p.R, groups = p.groups[MAX_SECTIONS - 1];
-  const int stride = inner_stride(total, 2), tall = (count + 15) / 16;
+  const int R16 = (R + 15) & ~15, wide = p.sections * p.R, tall = (count + 15) / 16;
   const bf16* b = reinterpret_cast<const bf16*>(p.b) + (long long)s * p.N * p.R;
-
-  constexpr int PIECES = sizeof(O) / 2;  // 16-byte pieces of eight columns
-  constexpr int HALVES = sizeof(O) == 2 ? 8 : 4;  // rows of a lane whose pieces are fetched a group ahead (of eight)
-  uint4 base[HALVES][PIECES];
-  Section sec{0, 0, 0};
-  int u0 = 0, col = -1;
-  uint2 w0[4];
-  const auto piece = [&](uint4 (&to)[PIECES], int h) {
-    const int r = rows[h * 8 + g];
-    if (r >= 0 && col >= 0) {
-      const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<const O*>(p.base) + r * p.base_stride + col);
+  const int left = blockIdx.x * stripe * PIECE, right = min(p.N, left + stripe * PIECE);
+  constexpr int ROW_BYTES = ACROSS * LIST * 128;
+  const int block = b_block(p.R), stage_bytes = ROW_BYTES + b_stage(p.R);
+  if (warp == WARPS) {
+    if (elect_one()) {
+      int slot = 0, turn = 0;
+      for (int c0 = left; c0 < right; c0 += PIECE) {
+        if (turn) tc::bar_wait(sm32(empty + slot), (turn - 1) & 1, p.err);
+        const uint32_t bar = sm32(filled + slot), at = sm32(ring) + slot * stage_bytes, b_bytes = min(PIECE, right - c0) * p.R * 2;
+        uint32_t bytes = b_bytes;
+        for (int i = 0; i < count; i += 32) bytes += ACROSS * (runs[i / 32] ? 32 : (min(32, count - i) + 3) / 4 * 4) * 128;
+        tc::bar_expect_tx(bar, bytes);
+        for (int i = 0; i < count; i += 32)
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) to[i] = at[i];
-    }
-  };
-  const auto find = [&](int gi) {
-    sec = section_of_group(p, gi);
-    u0 = gi * 32;
-    col = u0 + 8 * q < sec.width ? column(p, sec, u0 + 8 * q) : -1;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bf16* at = b_row(p, b, sec, u0, j);
-      w0[j] = at ? __ldg(reinterpret_cast<const uint2*>(at + 4 * q)) : make_uint2(0, 0);
-    }
-  };
-  int gi = blockIdx.x * each * WARPS + warp;
-  const int end = min(groups, (blockIdx.x + 1) * each * WARPS);
-  if (gi < end) {
-    find(gi);
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h) piece(base[h], h);
-  }
-  {
-    const bf16* inner = p.inner + ((long long)tile * SPLITS * LIST + r0) * wide;
-    const int pieces = total / 8;
-    for (int r = threadIdx.x / 8; r < SPLITS * ROWS; r += THREADS / 8) {
-      const int row = r % ROWS;
-      if (row >= tall * 16) continue;
-      const bf16* from = inner + ((long long)(r / ROWS) * LIST + row) * wide;
-      for (int i = threadIdx.x % 8; i < pieces; i += 8) {
-        // (sections of an adapter of a lower rank lie close together)
-        *reinterpret_cast<uint4*>(held + r * stride + i * 8) = row < count ? *reinterpret_cast<const uint4*>(from + i * 8) : make_uint4(0, 0, 0, 0);
+          for (int k = 0; k < ACROSS; ++k) {
+            const uint32_t to = at + (k * LIST + i) * 128;
+            if (runs[i / 32]) {
+              tc::tma_load_2d(to, &maps.run, c0 + k * COLUMNS, rows[i], bar);
+            } else {
+              for (int r = 0; r < 32 && i + r < count; r += 4) tma_gather4(to + r * 128, &maps.row, c0 + k * COLUMNS, rows[i + r], rows[i + r + 1], rows[i + r + 2], rows[i + r + 3], bar);
+            }
+          }
+        for (int i = 0; i < min(PIECE, right - c0) / 8; ++i) bulk_load(at + ROW_BYTES + i * block, b + (long long)(c0 + 8 * i) * p.R, 16 * p.R, bar);
+        if (++slot == stages) slot = 0, ++turn;
       }
     }
+    return;
   }
-  __syncthreads();
-  for (; gi < end; gi += WARPS) {
-    const bf16* mine = held + g * stride + sec.sec * R16 + 4 * q;
-    const bool more = gi + WARPS < end;
-    // 32 rows at a time
+  const bf16* inner = p.inner + ((long long)tile * SPLITS * LIST + g) * wide + 4 * q;
+  // What a warp does with a whole piece of one section is the same for every piece, and is worked out here (worked out anew each time,
+  // 346 instructions for 16 x 32 numbers, the kernel was bound by them: 1.2 TB/s).  Warp w has half w % 2 of the columns (a
+  // section's, where they alternate) and rows 16 (w / 2) on, and 64 further on.
+  const int half = warp & 1, own = p.alternating ? 16 * q + 8 * half : 32 * half + 8 * q;  // the lane's first column in the piece
+  int w_at[4];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (half * 2 >= tall) break;
-      float acc[2][4][4];
+  for (int j = 0; j < 4; ++j) w_at[j] = (p.alternating ? (g >> 1) * 2 + half : 4 * half + (g >> 1)) * (block / 2) + (2 * j + (g & 1)) * p.R;
+  const long long split = (long long)LIST * wide;
+  O* out[2][2];
+  int old_at[2][2];
+  const bf16* held[2];
+  bool live[2][2];
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+  for (int k = 0; k < 2; ++k) {
+    const int m = (warp >> 1) + 4 * k;
+    held[k] = inner + (long long)m * 16 * wide;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+    for (int h = 0; h < 2; ++h) {
+      const int r = m * 16 + 8 * h + g, byte = own * (int)sizeof(O);
+      live[k][h] = r < count;
+      out[k][h] = reinterpret_cast<O*>(p.out) + (live[k][h] ? rows[r] : 0) * p.out_stride + own;
+      old_at[k][h] = byte / 128 * LIST * 128 + (int)tc::sw128(r & (LIST - 1), byte % 128 / 16);
+    }
+  }
+  uint2 kept[2][KEPT][SPLITS][2];  // the first inner numbers of the section `kept_of`
+  int kept_of = -1;
+  int slot = 0, turn = 0;
+  for (int c0 = left; c0 < right; c0 += PIECE) {
+    int sec = p.alternating ? half : 0;
+    bool whole = right - c0 >= PIECE;
+    if (!p.alternating) {
+      const int from = c0 + 32 * half;
+      int end = p.width[0];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
-      for (int r = 0; r < R16; r += 16) {
-        uint2 w[4];
+      for (int i = 1; i < MAX_SECTIONS; ++i)
+        if (i < p.sections && from >= p.begin[i]) sec = i, end = p.begin[i] + p.width[i];
+      whole = whole && from + 32 <= end;
+    }
+    if (whole && sec != kept_of) {
+      kept_of = sec;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[j] = w0[j];
-          const bf16* at = r ? b_row(p, b, sec, u0, j) : nullptr;
-          if (r) w[j] = at ? __ldg(reinterpret_cast<const uint2*>(at + r + 4 * q)) : make_uint2(0, 0);
-        }
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          if (half * 2 + m < tall) {
+        for (int e = 0; e < KEPT; ++e)
 #pragma unroll
-            for (int i = 0; i < SPLITS; ++i) {
-              const bf16* h = mine + (i * ROWS + (half * 2 + m) * 16) * stride + r;
-              const uint2 lo = *reinterpret_cast<const uint2*>(h), hi = *reinterpret_cast<const uint2*>(h + 8 * stride);
+          for (int t = 0; t < SPLITS; ++t) {
+            const bf16* h = held[k] + t * split + sec * R16 + 16 * e;
+            kept[k][e][t][0] = live[k][0] && 16 * e < R16 ? *reinterpret_cast<const uint2*>(h) : make_uint2(0, 0);
+            kept[k][e][t][1] = live[k][1] && 16 * e < R16 ? *reinterpret_cast<const uint2*>(h + 8 * wide) : make_uint2(0, 0);
+          }
+    }
+    tc::bar_wait(sm32(filled + slot), turn & 1, p.err);
+    const char* at = ring + slot * stage_bytes;
+    if (whole) {
+      const bf16* bs = reinterpret_cast<const bf16*>(at + ROW_BYTES) + 4 * q;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) mma(acc[m][j], lo.x, hi.x, lo.y, hi.y, w[j].x, w[j].y);
+      for (int k = 0; k < 2; ++k) {
+        if ((warp >> 1) + 4 * k < tall) {
+          float acc[4][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+          const bf16* from = held[k] + sec * R16;
+          const auto step = [&](int r, auto inner_numbers) {
+            uint2 x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(bs + w_at[j] + r);
+#pragma unroll
+            for (int t = 0; t < SPLITS; ++t) {
+              uint2 lo, hi;
+              inner_numbers(t, lo, hi);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) mma(acc[j], lo.x, hi.x, lo.y, hi.y, x[j].x, x[j].y);
+            }
+          };
+#pragma unroll
+          for (int e = 0; e < KEPT; ++e)
+            if (16 * e < R16) step(16 * e, [&](int t, uint2& lo, uint2& hi) { lo = kept[k][e][t][0], hi = kept[k][e][t][1]; });
+          for (int r = 16 * KEPT; r < R16; r += 16)
+            step(r, [&](int t, uint2& lo, uint2& hi) {
+              lo = live[k][0] ? *reinterpret_cast<const uint2*>(from + t * split + r) : make_uint2(0, 0);
+              hi = live[k][1] ? *reinterpret_cast<const uint2*>(from + t * split + r + 8 * wide) : make_uint2(0, 0);
+            });
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (live[k][h]) {
+              uint4 old[sizeof(O) / 2];
+#pragma unroll
+              for (int e = 0; e < (int)sizeof(O) / 2; ++e) old[e] = *reinterpret_cast<const uint4*>(at + (old_at[k][h] ^ (16 * e)));  // (the next sixteen bytes of a swizzled row)
+              const float v[8] = {acc[0][2 * h], acc[0][2 * h + 1], acc[1][2 * h], acc[1][2 * h + 1], acc[2][2 * h], acc[2][2 * h + 1], acc[3][2 * h], acc[3][2 * h + 1]};
+              add_eight(old, out[k][h] + c0, v);
             }
           }
         }
       }
+      __syncwarp();
+      if (lane == 0) tc::bar_arrive(sm32(empty + slot));
+      if (++slot == stages) slot = 0, ++turn;
+      continue;
+    }
+    // a piece that the row ends in, or with the end of a section in it
+    const bf16* bs = reinterpret_cast<const bf16*>(at + ROW_BYTES) + 4 * q;
+    const int columns = min(PIECE, right - c0);
+    for (int u = warp; u < 2 * tall; u += WARPS) {
+      const int m = u >> 1;  // 16 rows; 32 columns, or those of a section where they alternate
+      const bool low = m * 16 + g < count, high = m * 16 + g + 8 < count;
+      const int from = p.alternating ? 0 : 32 * half;
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const int r = rows[half * 32 + h * 8 + g];
-        const int m = h / 2, e = h % 2 * 2;
-        const float v[8] = {acc[m][0][e], acc[m][0][e + 1], acc[m][1][e], acc[m][1][e + 1], acc[m][2][e], acc[m][2][e + 1], acc[m][3][e], acc[m][3][e + 1]};
-        if (r >= 0 && col >= 0) add_eight(base[(half * 4 + h) % HALVES], reinterpret_cast<O*>(p.out) + r * p.out_stride + col, v);
-        if (HALVES == 4 && half == 0) piece(base[h], 4 + h);
+      for (int i = 0; i < MAX_SECTIONS; ++i) {
+        // (32 columns may reach over the end of a section: each takes its own)
+        if (i >= p.sections || from >= columns || (p.alternating ? half != i : c0 + from >= p.begin[i] + p.width[i] || c0 + from + 32 <= p.begin[i])) continue;
+        // column 2q + e of the j-th of four tensor-core tiles is column 8q + 2j + e of the 32, so that a lane's eight results lie side by side
+        const bf16* w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = min(from + in_group(p, i, (g >> 1) * 8 + 2 * j + (g & 1)), columns - 1);  // (columns past the last are not written)
+          w[j] = bs + (c >> 3) * (block / 2) + (c & 7) * p.R;
+        }
+        float acc[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[j][k] = 0.f;
+        const bf16* held = inner + (long long)m * 16 * wide + i * R16;
+        for (int r = 0; r < R16; r += 16) {
+          uint2 x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(w[j] + r);
+#pragma unroll
+          for (int k = 0; k < SPLITS; ++k) {
+            const bf16* h = held + (long long)k * LIST * wide + r;
+            const uint2 lo = low ? *reinterpret_cast<const uint2*>(h) : make_uint2(0, 0), hi = high ? *reinterpret_cast<const uint2*>(h + 8 * wide) : make_uint2(0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma(acc[j], lo.x, hi.x, lo.y, hi.y, x[j].x, x[j].y);
+          }
+        }
+        const int c = from + in_group(p, i, 8 * q);
+        const bool mine = c < columns && (p.alternating || (c0 + c >= p.begin[i] && c0 + c < p.begin[i] + p.width[i]));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = m * 16 + g + 8 * h;
+          if (mine && r < count) {
+            uint4 old[sizeof(O) / 2];
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(O) / 2; ++k) {
+              const int byte = c * (int)sizeof(O) + 16 * k;
+              old[k] = *reinterpret_cast<const uint4*>(at + byte / 128 * LIST * 128 + tc::sw128(r, byte % 128 / 16));
+            }
+            const float v[8] = {acc[0][2 * h], acc[0][2 * h + 1], acc[1][2 * h], acc[1][2 * h + 1], acc[2][2 * h], acc[2][2 * h + 1], acc[3][2 * h], acc[3][2 * h + 1]};
+            add_eight(old, reinterpret_cast<O*>(p.out) + rows[r] * p.out_stride + c0 + c, v);
+          }
+        }
+        __syncwarp();  // (the next products take the whole warp)
       }
     }
-    if (more) {
-      find(gi + WARPS);
-#pragma unroll
-      for (int h = 0; h < HALVES; ++h) piece(base[h], h);
-    }
+    __syncwarp();
+    if (lane == 0) tc::bar_arrive(sm32(empty + slot));
+    if (++slot == stages) slot = 0, ++turn;
   }
 }
 
@@ -892,12 +983,15 @@ size_t few_smem(AdapterParams& p, int splits) {
   return rest + p.stage;
 }
 
-// Many rows: blocks of k that shared memory holds, columns of tensor memory, and the bytes for the ring and the sums (and 16 KB: the last lanes of
-// the accumulator read past the rows of A).
+// Many rows: blocks of k that shared memory holds, columns of tensor memory, and the bytes for the ring and the sums (16 KB at least: the last
+// lanes of the accumulator read past the rows of A).
 size_t many_smem(AdapterParams& p) {
-  const size_t rest = (size_t)CLUSTER * p.most * SUM_ROW * 4 + 16 * 1024, slot = slot_bytes(LIST, p.most), budget = 220 * 1024;
+  const size_t sums = (size_t)CLUSTER * p.most * SUM_ROW * 4, rest = max(sums, (size_t)16 * 1024), slot = slot_bytes(LIST, p.most);
   const int blocks = ((p.K + BLOCK_K - 1) / BLOCK_K + CLUSTER - 1) / CLUSTER;
-  p.slots = max(1, min(min((int)((budget - rest) / slot), MAX_SLOTS), blocks));
+  // Two CTAs an SM where that leaves three blocks each: with one, sixteen clusters of eight did not find room at the same time (a cluster
+  // lies within a GPC), and 2,048 rows took two rounds, 18 us for 10.
+  const int two = rest < 112 * 1024 ? (int)((112 * 1024 - rest) / slot) : 0, one = (int)((220 * 1024 - rest) / slot);
+  p.slots = max(1, min(min(two >= 3 ? two : one, MAX_SLOTS), blocks));
   p.tmem = LIST;
   return p.slots * slot + rest;
 }
@@ -924,19 +1018,31 @@ int make_maps(const AdapterParams& p, Maps& maps) {
 
 template <typename O, int SPLITS>
 int run_wide(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
-  const int total = p.sections * p.R, groups = p.groups[MAX_SECTIONS - 1];
-  const size_t one = many_smem(p), two = (size_t)SPLITS * ROWS * inner_stride(total, 2) * 2;
+  RowMaps base;
+  constexpr int COLUMNS = 128 / (int)sizeof(O);
+  for (int i = 0; i < 2; ++i) {
+    const cuuint64_t dims[2] = {(cuuint64_t)p.N, (cuuint64_t)p.n}, strides[1] = {(cuuint64_t)p.base_stride * sizeof(O)};
+    const cuuint32_t box[2] = {(cuuint32_t)COLUMNS, i ? 1u : 32u}, ones[2] = {1, 1};
+    if (tc::encode_tiled()(i ? &base.row : &base.run, sizeof(O) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(p.base), dims,
+                           strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return (int)cudaErrorInvalidValue;
+  }
+  const bool few_ranks = p.R <= 16;
+  const size_t one = many_smem(p), stage = (size_t)PIECE * sizeof(O) * LIST + (size_t)b_stage(p.R);
+  const int places = few_ranks ? 2 : 1;  // CTAs an SM: more inner numbers in registers leave room for one
+  const int stages = max(2, min(MAX_STAGES, (int)(220 * 1024 / places / stage)));
   const auto inner = adapter_inner_kernel<SPLITS>;
-  const auto outer = adapter_outer_kernel<O, SPLITS>;
+  const auto outer = few_ranks ? adapter_outer_kernel<O, SPLITS, 1> : adapter_outer_kernel<O, SPLITS, 4>;
   cudaError_t rc = cudaFuncSetAttribute(inner, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one);
-  if (rc == cudaSuccess) rc = cudaFuncSetAttribute(outer, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)two);
+  if (rc == cudaSuccess) rc = cudaFuncSetAttribute(outer, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages * stage));
   if (rc != cudaSuccess) return (int)rc;
   const int r = launch(inner, dim3(tiles * CLUSTER), dim3(THREADS), one, st, p, maps);
   if (r) return r;
-  // groups a warp: as many as leave about two CTAs for every SM
-  const int stripes = (groups + WARPS - 1) / WARPS, blocks = (p.n + ROWS - 1) / ROWS;
-  const int each = max(1, min(8, (int)((long long)stripes * blocks / (2 * 148))));
-  return launch(outer, dim3((stripes + each - 1) / each, tiles * (LIST / ROWS)), dim3(THREADS), two, st, p, each);
+  // pieces of a CTA: as many as leave a CTA for every place there is
+  const int pieces = (p.N + PIECE - 1) / PIECE, full = (p.n + LIST - 1) / LIST;
+  const int stripe = max(1, min(pieces, (int)(((long long)pieces * full + places * 148 - 1) / (places * 148))));
+  return launch(outer, dim3((pieces + stripe - 1) / stripe, tiles), dim3(THREADS + 32), stages * stage, st, p, base, stripe, stages);
 }
 
 // ---- the rows of a step by adapter: one CTA.  Rows without an adapter come last.  The rows of an adapter keep their order within a
@@ -1059,7 +1165,6 @@ int run(AdapterParams& p, const int* ends, int wide, int max_tiles, int two, cud
     const int end = i < p.sections - 1 ? ends[i] : p.N;
     p.begin[i] = p.alternating ? 0 : from;
     p.width[i] = i >= p.sections ? 0 : p.alternating ? p.N / 2 : end - from;
-    p.groups[i] = (i ? p.groups[i - 1] : 0) + (p.width[i] + 31) / 32;
     from = end;
   }
   p.most = min(p.sections, MOST / p.R) * p.R;
@@ -1080,7 +1185,7 @@ int run(AdapterParams& p, const int* ends, int wide, int max_tiles, int two, cud
   KVF_API int kvf_adapter_add_##SUF(const void* x, long long x_stride, const void* a, const void* b, const float* scales, const int* ranks, const int* ids, int n, int S,  \
                                     int sections, int R, int K, int N, int end0, int end1, int end2, int alternating, const void* base, long long base_stride, void* out,  \
                                     long long out_stride, int wide, const int* rows, const int* tiles, int max_tiles, void* inner, int two, int* err, cudaStream_t st) {   \
-    AdapterParams p{x, a, b, scales, ranks, ids, rows, tiles, (bf16*)inner, base, out, err, x_stride, base_stride, out_stride, n, S, sections, R, K, N, {}, {}, {}, alternating, 0, 0, 0, 0}; \
+    AdapterParams p{x, a, b, scales, ranks, ids, rows, tiles, (bf16*)inner, base, out, err, x_stride, base_stride, out_stride, n, S, sections, R, K, N, {}, {}, alternating, 0, 0, 0, 0}; \
     const int ends[3] = {end0, end1, end2};                                                                                                                               \
     return run<T, WIDE_SPLITS>(p, ends, wide, max_tiles, two, st);                                                                                                             \
   }
