@@ -15,7 +15,7 @@ import os as _os
 # KiB) unless the caller has said otherwise.
 _os.environ.setdefault("CUBLASLT_WORKSPACE_SIZE", "65536")
 
-from .config.engine_config import CacheConfig, EngineConfig, SchedulerConfig  # noqa: E402
+from .config.engine_config import AdapterConfig, CacheConfig, EngineConfig, SchedulerConfig  # noqa: E402
 from .config.model_config import ConfigError, ModelConfig, RopeScaling
 from .config.registry import PRESETS, register_architecture
 from .engine.request import FinishReason, Request, RequestOutput, RequestStatus
@@ -25,6 +25,8 @@ __version__ = "0.1.0"
 
 __all__ = [
     "PRESETS",
+    "AdapterConfig",
+    "BeamParams",
     "CacheConfig",
     "ConfigError",
     "EngineConfig",
@@ -50,6 +52,10 @@ def __getattr__(name):
         from .engine.engine import InferenceEngine
 
         return InferenceEngine
+    if name == "BeamParams":
+        from .engine.beam import BeamParams
+
+        return BeamParams
     if name == "ByteTokenizer":
         from .engine.tokenizer import ByteTokenizer
 

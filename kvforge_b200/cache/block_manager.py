@@ -6,7 +6,10 @@ in what the scheduler sees: ``can_allocate`` / ``allocate`` at admission (with a
 ``can_append_slots`` / ``append_slots`` for every running request every step, ``free`` when a
 request ends, is aborted or is preempted; a last-in-first-out free list whose block 0 is
 handed out first (block_manager.py:73-74), so freed pages are the first used again.
-Left out: sharing (fork, copy-on-write) and the prefix cache.
+Left out: the prefix cache.
+
+``fork`` gives a request's pages to a second one (beams): full pages are shared and counted, the last, partly filled
+page becomes a copy, so that whoever writes next writes a page of its own.
 
 Added: cache *groups*.  Layers that keep the same thing per token form a group with pages
 and tables of its own.  A ``full`` group keeps every key.  A ``window`` group keeps the last
@@ -64,7 +67,7 @@ class _Pool:
         self.spec = spec
         self.num_blocks = num_blocks
         self.free: list[int] = list(range(num_blocks - 1, -1, -1))
-        self.held = [False] * num_blocks
+        self.held = [0] * num_blocks  # in how many tables a page is
         self.tables: dict[str, list[int]] = {}
         # the same tables as int32 arrays (with room to grow), so that a step copies a table instead of converting a list
         self.arrays: dict[str, np.ndarray] = {}
@@ -82,7 +85,7 @@ class _Pool:
         if not self.free:
             raise NoFreeBlocksError("KV cache exhausted")
         b = self.free.pop()
-        self.held[b] = True
+        self.held[b] = 1
         return b
 
     def take(self, n: int) -> list[int]:
@@ -94,14 +97,20 @@ class _Pool:
         pages = self.free[: -n - 1 : -1]
         del self.free[-n:]
         for b in pages:
-            self.held[b] = True
+            self.held[b] = 1
         return pages
+
+    def share(self, b: int) -> None:
+        if b < 0 or b >= self.num_blocks or not self.held[b]:
+            raise RuntimeError(f"block {b} is not held, so it cannot be shared")
+        self.held[b] += 1
 
     def release(self, b: int) -> None:
         if b < 0 or b >= self.num_blocks or not self.held[b]:
             raise RuntimeError(f"double free of block {b}")
-        self.held[b] = False
-        self.free.append(b)
+        self.held[b] -= 1
+        if not self.held[b]:
+            self.free.append(b)
 
 
 class BlockManager:
@@ -197,7 +206,7 @@ class BlockManager:
         kept = min(self._kept_blocks(pool), first)
         live = [i for i in range(want) if i < kept or i >= first]
         take = sum(1 for i in live if i >= len(table) or table[i] < 0)
-        back = sum(1 for i in range(kept, min(first, len(table))) if table[i] >= 0)
+        back = sum(1 for i in range(kept, min(first, len(table))) if table[i] >= 0 and pool.held[table[i]] == 1)
         return take, back
 
     def can_ever_fit(self, num_tokens: int, max_portion: int) -> bool:
@@ -288,6 +297,40 @@ class BlockManager:
         self._num_tokens[seq_id] = max(self._num_tokens[seq_id], total_tokens)
         return []
 
+    # ------------------------------------------------------------------ sharing
+    def fork_demand(self, num_tokens: int) -> int:
+        """Pages of a group that a fork of a request with ``num_tokens`` computed tokens takes."""
+        return 1 if num_tokens % self.block_size else 0
+
+    def fork(self, seq_id: str, child_id: str, num_tokens: int) -> list[tuple[int, int, int, int]]:
+        """A second request with the first ``num_tokens`` tokens of ``seq_id``: full pages are shared, the page that is
+        partly filled is one of the child's own.  Returns the copies to make before either writes again: (group,
+        source page, target page, positions)."""
+        if seq_id not in self._num_tokens:
+            raise KeyError(f"sequence {seq_id} has no tables")
+        if child_id in self._num_tokens:
+            raise ValueError(f"sequence {child_id} already allocated")
+        if num_tokens < 0 or any(self.blocks_needed(num_tokens) > len(p.tables[seq_id]) for p in self._pools):
+            raise ValueError(f"sequence {seq_id} does not hold {num_tokens} tokens")
+        full, rest = divmod(num_tokens, self.block_size)
+        if rest and any(not p.free for p in self._pools if p.tables[seq_id][full] >= 0):
+            raise NoFreeBlocksError(f"cannot fork {seq_id}")
+        copies = []
+        for gi, pool in enumerate(self._pools):
+            table = pool.tables[seq_id][:full]
+            for b in table:
+                if b >= 0:
+                    pool.share(b)
+            if rest:
+                last = pool.tables[seq_id][full]
+                table.append(pool.pop() if last >= 0 else RELEASED)
+                if last >= 0:
+                    copies.append((gi, last, table[-1], rest))
+            pool.tables[child_id] = table
+            pool.arrays[child_id] = np.array(table, dtype=np.int32)
+        self._num_tokens[child_id] = num_tokens
+        return copies
+
     def mark_computed(self, seq_id: str, num_tokens: int) -> None:
         """Record the live token count (block_manager.py:249-266, without the prefix hashes)."""
         if seq_id in self._num_tokens:
@@ -308,18 +351,19 @@ class BlockManager:
 
     # ------------------------------------------------------------------ checks and figures
     def check_invariants(self) -> None:
-        """Every page is free or in exactly one table, never both, never twice."""
+        """Every page is free or in as many tables as it is counted for, never both, never twice in one."""
         for gi, pool in enumerate(self._pools):
-            seen: dict[int, str] = {}
+            seen: dict[int, list[str]] = {}
             for seq, table in pool.tables.items():
                 if pool.arrays[seq][: len(table)].tolist() != table:
                     raise AssertionError(f"group {gi}: the table of {seq} and its array differ")
                 for b in table:
                     if b < 0:
                         continue
-                    if b in seen:
-                        raise AssertionError(f"group {gi}: block {b} held by {seen[b]} and {seq}")
-                    seen[b] = seq
+                    holders = seen.setdefault(b, [])
+                    if holders and (seq in holders or len(holders) >= pool.held[b]):
+                        raise AssertionError(f"group {gi}: block {b} held by {holders[0]} and {seq}")
+                    holders.append(seq)
             free = set(pool.free)
             if len(free) != len(pool.free):
                 raise AssertionError(f"group {gi}: a block is on the free list twice")
@@ -328,7 +372,7 @@ class BlockManager:
             if len(free) + len(seen) != pool.num_blocks:
                 raise AssertionError(f"group {gi}: {pool.num_blocks - len(free) - len(seen)} blocks lost")
             for b in range(pool.num_blocks):
-                if pool.held[b] != (b in seen):
+                if pool.held[b] != len(seen.get(b, ())):
                     raise AssertionError(f"group {gi}: held flag of block {b} is wrong")
 
     @property
@@ -341,12 +385,13 @@ class BlockManager:
         """Figures of the first group (block_manager.py:288-314)."""
         pool = self._pools[0]
         used = pool.num_blocks - len(pool.free)
-        tokens = 0
+        filled: dict[int, int] = {}  # a page that several requests share counts once
         for seq, table in pool.tables.items():
             n = self._num_tokens.get(seq, 0)
             for i, b in enumerate(table):
                 if b >= 0:
-                    tokens += min(self.block_size, max(0, n - i * self.block_size))
+                    filled[b] = max(filled.get(b, 0), min(self.block_size, max(0, n - i * self.block_size)))
+        tokens = sum(filled.values())
         slots = used * self.block_size
         return BlockManagerStats(
             num_blocks=self.num_blocks,

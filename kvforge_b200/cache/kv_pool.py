@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 
+from .. import ops
 from ..parts.base import LayerCache
 
 
@@ -28,6 +29,7 @@ class KVPool:
         self.states: list[torch.Tensor | None] = []
         for shape in model.state_shapes:
             self.states.append(None if shape is None else torch.zeros((num_slots, *shape), dtype=torch.float32, device=device))
+        self._state_table: ops.StateTable | None = None
         self.caches: list[LayerCache | None] = []
         for idx, call in enumerate(model.spec.execution):
             owner = model.call_group[idx if call.kv_from is None else call.kv_from]
@@ -52,6 +54,25 @@ class KVPool:
         for st in self.states:
             if st is not None:
                 st[slots] = 0
+
+    def copy_pages(self, copies: list[tuple[int, int, int, int]]) -> None:
+        """(group, source page, target page, positions) as ``BlockManager.fork`` returns them: one launch a group, every layer."""
+        for gi, k in enumerate(self.k):
+            rows = [c[1:] for c in copies if c[0] == gi]
+            if rows:
+                src, dst, tokens = torch.tensor(rows, dtype=torch.int32).t().contiguous().to(k.device)
+                v = self.v[gi]
+                ops.copy_pages(k, None if v is k else v, src, dst, tokens)
+
+    def copy_states(self, copies: list[tuple[int, int]]) -> None:
+        """(source slot, target slot): every mixer's state, one launch."""
+        states = [t for t in self.states if t is not None]
+        if not copies or not states:
+            return
+        if self._state_table is None:
+            self._state_table = ops.StateTable(states)
+        src, dst = torch.tensor(copies, dtype=torch.int32).t().contiguous().to(states[0].device)
+        ops.copy_states(self._state_table, src, dst)
 
 
 def bytes_per_block(model, block_size: int, dtype: torch.dtype) -> int:

@@ -35,14 +35,18 @@ class StateSlotPool:
     def slot(self, seq_id: str) -> int:
         return self._of[seq_id]
 
-    def allocate(self, seq_id: str) -> int:
+    def allocate(self, seq_id: str, fresh: bool = True) -> int:
+        """``fresh=False``: the slot's state is not cleared (the caller writes all of it)."""
         if seq_id in self._of:
             raise ValueError(f"sequence {seq_id} already holds a state slot")
         if not self._free:
             raise NoFreeSlotsError("no free state slot")
         s = self._free.pop()
         self._of[seq_id] = s
-        self.fresh.append(s)
+        if fresh:
+            self.fresh.append(s)
+        else:  # (it may have been handed out and given back since the last step)
+            self.fresh = [t for t in self.fresh if t != s]
         return s
 
     def free(self, seq_id: str) -> None:

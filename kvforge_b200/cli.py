@@ -4,7 +4,8 @@ The options that umarhassan-cloud/kvforge's launcher has (scripts/serve.py:41-61
 names and meanings: ``--preset`` / ``--hf-model`` (here a local folder with config.json and
 safetensors), ``--device``, ``--dtype``, ``--block-size``, ``--num-blocks``, ``--kv-cache-gb``,
 ``--max-num-seqs``, ``--max-num-batched-tokens``, ``--max-model-len``.  The sampling options are
-the fields of its ``SamplingParams``.  Prompts are token ids (``--prompt-ids "1,2,3"``, one
+the fields of its ``SamplingParams``.  ``--adapter`` runs all prompts with the low-rank adapter in a folder; ``--num-beams`` searches for
+the likeliest continuations instead of sampling.  Prompts are token ids (``--prompt-ids "1,2,3"``, one
 per use, or ``--prompt-file`` with one comma-separated prompt a line) or, with the byte
 tokenizer of the random-weight demos, text (``--prompt``).
 
@@ -21,7 +22,7 @@ from pathlib import Path
 
 
 def main() -> int:
-    from . import PRESETS, ByteTokenizer, CacheConfig, EngineConfig, InferenceEngine, SamplingParams, SchedulerConfig
+    from . import PRESETS, AdapterConfig, BeamParams, ByteTokenizer, CacheConfig, EngineConfig, InferenceEngine, SamplingParams, SchedulerConfig
 
     p = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     src = p.add_mutually_exclusive_group()
@@ -44,6 +45,9 @@ def main() -> int:
     p.add_argument("--top-k", type=int, default=0)
     p.add_argument("--top-p", type=float, default=1.0)
     p.add_argument("--ignore-eos", action="store_true")
+    p.add_argument("--adapter", help="folder of a low-rank adapter (adapter_config.json and safetensors)")
+    p.add_argument("--num-beams", type=int, default=0, help="beam search with so many beams (0: sampling)")
+    p.add_argument("--length-penalty", type=float, default=1.0)
     p.add_argument("--stats", action="store_true", help="print the engine's figures after the run")
     args = p.parse_args()
 
@@ -80,13 +84,25 @@ def main() -> int:
         device=args.device,
         dtype=args.dtype,
         seed=args.seed,
+        adapters=AdapterConfig(max_adapters=1, max_rank=128) if args.adapter else None,
     )
     engine = InferenceEngine(config, model=args.hf_model, tokenizer=tokenizer)
     kv = engine.kv_cache
     name = args.hf_model or f"kvforge_b200-{args.preset}-random"
     print(f"kvforge_b200: model={name} blocks={kv.num_blocks}x{kv.block_size} kv={kv.memory_bytes / 2**20:.1f} MiB device={args.device}", file=sys.stderr)
+    if args.adapter:
+        engine.load_adapter("adapter", args.adapter)
+    adapter = "adapter" if args.adapter else None
+    if args.num_beams:
+        bp = BeamParams(num_beams=args.num_beams, max_tokens=args.max_tokens, length_penalty=args.length_penalty, num_return=args.num_beams, ignore_eos=args.ignore_eos)
+        for found in engine.beam_search(prompts, bp, adapters=adapter):
+            print(json.dumps({"prompt_token_ids": found.prompt_token_ids, "hypotheses": [
+                {"output_token_ids": h.token_ids, "score": h.score, "finish_reason": h.finish_reason.value, "text": h.text} for h in found.hypotheses]}))  # fmt: skip
+        if args.stats:
+            print(json.dumps(engine.stats(), default=str), file=sys.stderr)
+        return 0
     sp = SamplingParams(max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, ignore_eos=args.ignore_eos)
-    for out in engine.generate(prompts, sp):
+    for out in engine.generate(prompts, sp, adapters=adapter):
         print(json.dumps({"request_id": out.request_id, "prompt_token_ids": out.prompt_token_ids, "output_token_ids": out.output_token_ids,
                           "finish_reason": out.finish_reason.value if out.finish_reason else None, "text": out.text}))  # fmt: skip
     if args.stats:

@@ -63,6 +63,21 @@ class SchedulerConfig:
 
 
 @dataclass
+class AdapterConfig:
+    """Room for low-rank adapters that requests name (``InferenceEngine.load_adapter``): how many are loaded at a time, and the
+    highest rank of one.  Not in umarhassan-cloud/kvforge."""
+
+    max_adapters: int = 8
+    max_rank: int = 16
+
+    def __post_init__(self) -> None:
+        if not 1 <= self.max_adapters <= 4096:
+            raise ValueError("max_adapters must be between 1 and 4,096")
+        if not 1 <= self.max_rank <= 128:
+            raise ValueError("max_rank must be between 1 and 128")
+
+
+@dataclass
 class EngineConfig:
     """src/tokenvault/config.py:134-151.  ``model`` may be left ``None`` when the engine is
     given a model folder."""
@@ -78,6 +93,8 @@ class EngineConfig:
     # Read a step's tokens while the next step runs (a decoded token feeds the next step on the
     # device; stop tokens are seen one step late).  False: read them before the next step.
     async_output: bool = True
+    # Low-rank adapters that requests may name; None: none can be loaded, and nothing is kept for them.
+    adapters: AdapterConfig | None = None
 
     def __post_init__(self) -> None:
         self.dtype = parse_dtype(self.dtype)

@@ -16,9 +16,10 @@ import torch
 from ..cache.block_manager import BlockManager, GroupSpec
 from ..cache.kv_pool import KVPool, bytes_per_block
 from ..cache.state_slots import StateSlotPool
-from ..config.engine_config import CacheConfig, parse_dtype
+from ..config.engine_config import AdapterConfig, CacheConfig, parse_dtype
 from ..config.model_config import read_config_json
 from ..config.registry import architecture_of, get_architecture
+from ..parts.adapters import AdapterStore
 from ..parts.model import DecoderModel, ModelSpec
 from ..weights.loader import load_weights
 from ..weights.random_init import random_weights
@@ -63,6 +64,7 @@ class EngineCore:
         cuda_graphs: bool = False,
         lazy_buffers: bool = False,
         pdl: bool | None = None,
+        adapters: AdapterConfig | None = None,
     ) -> None:
         if not torch.cuda.is_available():
             raise RuntimeError("kvforge_b200 needs a CUDA device: there is no CPU path")
@@ -76,6 +78,8 @@ class EngineCore:
         cache = cache or CacheConfig()
         self.model = DecoderModel(spec)
         self.rt = Runtime(self.device, self.dtype, max_num_batched_tokens, max_num_seqs, self.max_model_len, lazy=lazy_buffers)
+        if adapters is not None:
+            self.rt.adapters = AdapterStore(adapters.max_adapters, adapters.max_rank, max_num_batched_tokens, self.dtype, self.device)
         expected = self.model.expected_weights()
         if model_dir is not None:
             weights = load_weights(model_dir, expected, self.dtype, self.device, spec.ignore_suffixes)

@@ -22,8 +22,10 @@ from typing import Any
 import torch
 
 from ..config.engine_config import EngineConfig
+from ..parts.adapters import AdapterError, read_adapter
 from ..sampling.params import SamplingParams
 from ..sampling.sampler import Sampler, request_stream_base
+from .beam import BeamOutput, BeamParams, BeamSearch
 from .core import EngineCore, spec_from_config, spec_from_model_dir
 from .metrics import MetricsCollector
 from .request import FinishReason, Request, RequestOutput
@@ -75,6 +77,7 @@ class InferenceEngine:
             max_num_batched_tokens=sc.max_num_batched_tokens,
             max_model_len=sc.max_model_len,
             cuda_graphs=config.cuda_graphs,
+            adapters=config.adapters,
         )
         self.block_manager = self.core.block_manager
         self.kv_cache = self.core.pool
@@ -109,15 +112,18 @@ class InferenceEngine:
         sampling_params: SamplingParams | None = None,
         request_id: str | None = None,
         arrival_time: float | None = None,
+        adapter: str | None = None,
     ) -> str:
         """Queue a prompt (text or token ids) and return the request's name (engine.py:106-134).
-        The scheduler refuses what can never run (``RequestRejectedError``)."""
+        The scheduler refuses what can never run (``RequestRejectedError``).  ``adapter``: the name of a loaded low-rank
+        adapter that the request runs with."""
+        slot = self._adapter_slot(adapter)
         ids = self._token_ids(prompt)
         name = request_id if request_id else f"req-{next(self._ids)}"
         params = sampling_params if sampling_params is not None else SamplingParams()
         eos = getattr(self.tokenizer, "eos_token_id", None) if self.tokenizer is not None else self.core.spec.eos_token_id
         self.scheduler.add_request(
-            Request(name, ids, params, arrival_time, eos, stream_base=request_stream_base(self.config.seed, name, params))
+            Request(name, ids, params, arrival_time, eos, stream_base=request_stream_base(self.config.seed, name, params), adapter=adapter, adapter_slot=slot)
         )
         return name
 
@@ -132,20 +138,81 @@ class InferenceEngine:
         self.metrics.record_finished(req)
         return True
 
+    # ------------------------------------------------------------------ adapters
+    def _adapter_slot(self, name: str | None) -> int:
+        if name is None:
+            return -1
+        return self._adapter_store().slot(name)
+
+    def _adapter_store(self):
+        if self.core.rt.adapters is None:
+            raise AdapterError("this engine keeps no adapters (EngineConfig.adapters)")
+        return self.core.rt.adapters
+
+    def load_adapter(self, name: str, source: str | Path | dict[str, torch.Tensor], scale: float | None = None) -> None:
+        """Load a low-rank adapter under ``name``: a folder with ``adapter_config.json`` and safetensors, or the tensors by name
+        (``<projection>.lora_A.weight``, ``<projection>.lora_B.weight``) with their ``scale``."""
+        store = self._adapter_store()
+        if isinstance(source, dict):
+            tensors, own = source, 1.0
+        else:
+            tensors, own = read_adapter(source)
+        store.load(name, tensors, own if scale is None else float(scale))
+
+    def unload_adapter(self, name: str) -> None:
+        """Give an adapter's place back; refused while a request runs with it."""
+        store = self._adapter_store()
+        if any(r.adapter == name for r in self.scheduler.requests.values()):
+            raise AdapterError(f"adapter {name!r} is in use")
+        store.unload(name)
+
+    def _per_prompt(self, adapters: str | Sequence[str | None] | None, count: int) -> list[str | None]:
+        if adapters is None or isinstance(adapters, str):
+            return [adapters] * count
+        if len(adapters) != count:
+            raise ValueError(f"{len(adapters)} adapters for {count} prompts")
+        return list(adapters)
+
+    # ------------------------------------------------------------------ beams
+    def beam_search(
+        self,
+        prompts: Sequence[str | Sequence[int]],
+        params: BeamParams | None = None,
+        adapters: str | Sequence[str | None] | None = None,
+    ) -> list[BeamOutput]:
+        """The likeliest continuations of every prompt (``engine/beam.py``); one output per prompt, in the order given.  The engine must
+        have no unfinished requests.  ``adapters``: one for all, or one per prompt."""
+        if self.has_unfinished_requests():
+            raise RuntimeError("beam search needs the engine to itself: finish or abort the queued requests first")
+        params = params if params is not None else BeamParams()
+        self._resolve(self._take_pending())
+        slots = [self._adapter_slot(a) for a in self._per_prompt(adapters, len(prompts))]
+        ids = [self._token_ids(p) for p in prompts]
+        eos = getattr(self.tokenizer, "eos_token_id", None) if self.tokenizer is not None else self.core.spec.eos_token_id
+        stops = set() if params.ignore_eos else {t for t in (eos, *params.stop_token_ids) if t is not None}
+        outputs = BeamSearch(self, params, slots).run(ids, stops)
+        if self.tokenizer is not None:
+            for out in outputs:
+                for h in out.hypotheses:
+                    h.text = self.tokenizer.decode(h.token_ids)
+        return outputs
+
     def generate(
         self,
         prompts: Sequence[str | Sequence[int]],
         sampling_params: SamplingParams | Sequence[SamplingParams] | None = None,
+        adapters: str | Sequence[str | None] | None = None,
     ) -> list[RequestOutput]:
         """Run all prompts to their end; one output per prompt, in the order given
-        (engine.py:145-159).  ``sampling_params``: one for all, or one per prompt."""
+        (engine.py:145-159).  ``sampling_params`` and ``adapters``: one for all, or one per prompt."""
         if isinstance(sampling_params, SamplingParams) or sampling_params is None:
             per_prompt = [sampling_params] * len(prompts)
         else:
             per_prompt = list(sampling_params)
             if len(per_prompt) != len(prompts):
                 raise ValueError(f"{len(per_prompt)} sampling parameter sets for {len(prompts)} prompts")
-        names = [self.add_request(prompt, sp) for prompt, sp in zip(prompts, per_prompt)]
+        chosen = self._per_prompt(adapters, len(prompts))
+        names = [self.add_request(prompt, sp, adapter=a) for prompt, sp, a in zip(prompts, per_prompt, chosen)]
         final: dict[str, RequestOutput] = {}
         while self.has_unfinished_requests():
             final.update((out.request_id, out) for out in self.step() if out.finished)
@@ -208,9 +275,9 @@ class InferenceEngine:
             if previous is not None and s.num_new_tokens == 1 and r.has_token_in_flight:
                 row = previous.rows.get(r.request_id)
             if row is not None:
-                items.append(BatchItem(r.request_id, [0], start, want, feedback_row=row))
+                items.append(BatchItem(r.request_id, [0], start, want, feedback_row=row, adapter=r.adapter_slot))
             else:
-                items.append(BatchItem(r.request_id, r.tokens(start, s.num_new_tokens), start, want))
+                items.append(BatchItem(r.request_id, r.tokens(start, s.num_new_tokens), start, want, adapter=r.adapter_slot))
             if completes:
                 sampled.append(r)
         logits = self.runner.step(items)

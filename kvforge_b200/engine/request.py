@@ -50,7 +50,7 @@ class Request:
     __slots__ = (
         "request_id", "prompt_token_ids", "sampling_params", "arrival_time", "eos_token_id", "stream_base",
         "status", "finish_reason", "output_token_ids", "num_computed_tokens", "num_preemptions",
-        "first_scheduled_time", "finish_time", "token_times", "_prompt_array",
+        "first_scheduled_time", "finish_time", "token_times", "_prompt_array", "adapter", "adapter_slot",
     )  # fmt: skip
 
     def __init__(
@@ -61,8 +61,11 @@ class Request:
         arrival_time: float | None = None,
         eos_token_id: int | None = None,
         stream_base: int = 0,
+        adapter: str | None = None,
+        adapter_slot: int = -1,
     ) -> None:
         self.request_id = request_id
+        self.adapter, self.adapter_slot = adapter, adapter_slot  # the low-rank adapter it runs with
         self.prompt_token_ids = prompt_token_ids
         self.sampling_params = sampling_params if sampling_params is not None else SamplingParams()
         self.arrival_time = time.perf_counter() if arrival_time is None else arrival_time

@@ -36,6 +36,7 @@ class Runtime:
         self.capturing = False
         self.graphs_captured = False  # captured graphs hold buffer addresses: no buffer may move afterwards
         self._side: torch.cuda.Stream | None = None
+        self.adapters = None  # a ``parts.adapters.AdapterStore`` where requests may bring low-rank adapters
 
     def side_stream(self) -> torch.cuda.Stream:
         """A second stream for a kernel that may run beside the step's chain while a step is captured
@@ -75,6 +76,8 @@ class Runtime:
                 what.append("a cache slot outside the pool")
             if flag & 4:
                 what.append("a bounded wait inside a kernel ran out")
+            if flag & 32:
+                what.append("an adapter outside the bank")
             if flag & 16:
                 what.append("a position beyond the model's table of positions")
             raise RuntimeError("device-side check failed: " + ", ".join(what or [f"flag {flag}"]))
@@ -127,6 +130,10 @@ class StepContext:
     context_bound: int = 0
     # Per registered tile size a ``QueryTiles``.  Empty when every sequence brings one token.
     query_tiles: dict = field(default_factory=dict)
+    # The adapter of every token, or -1: [N]; ``None`` in a step that has none.  ``adapters`` (``ops.AdapterGroups``): the tokens by
+    # adapter, made of it before the blocks run.
+    adapter_ids: torch.Tensor | None = None
+    adapters: object | None = None
     extras: dict = field(default_factory=dict)
 
     @property

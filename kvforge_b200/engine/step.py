@@ -52,6 +52,7 @@ class BatchItem:
     # For a single token that the device sampled in the step before and the host has not read
     # yet: its row in the runner's ``token_feedback`` buffer (``token_ids`` is then ignored).
     feedback_row: int | None = None
+    adapter: int = -1  # slot of the low-rank adapter that the request runs with
 
     def wanted(self) -> list[int]:
         n = len(self.token_ids)
@@ -84,6 +85,7 @@ class _Layout:
     n_groups: int
     r_cap: int
     tile_sizes: tuple[int, ...] = ()
+    adapters: bool = False  # whether the step says which adapter a token takes
     off: dict[str, int] = field(default_factory=dict)
     total: int = 0
 
@@ -93,6 +95,7 @@ class _Layout:
             ("token_ids", self.n_cap),
             ("positions", self.n_cap),
             ("feedback_rows", self.n_cap),
+            *((("adapter_ids", self.n_cap),) if self.adapters else ()),
             ("logit_rows", self.r_cap),
             ("qsl", self.b_cap + 1),
             ("ctx", self.b_cap),
@@ -140,7 +143,7 @@ class ModelRunner:
         # the most sequences a step can hold is a bucket of its own, so that no batch size goes without a graph
         self.graph_buckets = sorted({b for b in graph_buckets if b <= rt.max_seqs} | ({rt.max_seqs} if rt.max_seqs <= max(graph_buckets) else set())) or [rt.max_seqs]
         # keyed by (tokens, sequences, longest context the graph reaches, single-token sequences in a step of
-        # many tokens, decode form); the form is part of the key because a step of many tokens padded to as many
+        # many tokens, decode form, adapters); the form is part of the key because a step of many tokens padded to as many
         # tokens as sequences (64 tokens in 64 sequences) is another graph than 64 decoding sequences
         self._graphs: dict[tuple, tuple[torch.cuda.CUDAGraph, torch.Tensor]] = {}
         self.graph_kernels: dict[tuple, int] = {}  # kernels of this library inside each captured graph
@@ -163,7 +166,7 @@ class ModelRunner:
 
     # ------------------------------------------------------------------ buffers
     def _layout(self, n_cap: int, b_cap: int, width: int, r_cap: int) -> _Layout:
-        return _Layout(n_cap, b_cap, max(1, width), self.n_groups, max(1, r_cap), tuple(sorted(self.rt.query_tile_sizes)))
+        return _Layout(n_cap, b_cap, max(1, width), self.n_groups, max(1, r_cap), tuple(sorted(self.rt.query_tile_sizes)), self.rt.adapters is not None)
 
     def _ensure(self, total: int) -> None:
         if total <= self._cap:
@@ -203,6 +206,8 @@ class ModelRunner:
             host[o["token_ids"] : o["token_ids"] + lay.n_cap] = 0
             host[o["positions"] : o["positions"] + lay.n_cap] = 0
             host[o["feedback_rows"] : o["feedback_rows"] + lay.n_cap] = -1
+            if lay.adapters:
+                host[o["adapter_ids"] : o["adapter_ids"] + lay.n_cap] = -1
             host[o["logit_rows"] : o["logit_rows"] + lay.r_cap] = 0
             host[o["slots"] : o["slots"] + self.n_groups * lay.n_cap] = -1
         n = 0
@@ -231,6 +236,8 @@ class ModelRunner:
                     raise ValueError("a token fed back on the device must be a single token, and a feedback buffer must be set")
                 host[o["token_ids"] + n] = 0
                 host[o["feedback_rows"] + n] = item.feedback_row
+            if lay.adapters:
+                host[o["adapter_ids"] + n : o["adapter_ids"] + n + k] = item.adapter
             host[o["positions"] + n : o["positions"] + n + k] = np.arange(item.start_pos, end, dtype=np.int32)
             for g in range(self.n_groups):
                 base = o["slots"] + g * lay.n_cap + n
@@ -284,6 +291,8 @@ class ModelRunner:
         pos = np.array(starts, dtype=np.int32)
         for name, values in (("token_ids", tokens), ("feedback_rows", feedback), ("positions", pos), ("ctx", pos + 1), ("state_slots", slots)):
             host[o[name] : o[name] + nb] = values
+        if lay.adapters:
+            host[o["adapter_ids"] : o["adapter_ids"] + nb] = [item.adapter for item in items]
         host[o["qsl"] : o["qsl"] + nb + 1] = np.arange(nb + 1, dtype=np.int32)
         for g in range(self.n_groups):
             at = o["tables"] + g * lay.b_cap * lay.width
@@ -332,7 +341,9 @@ class ModelRunner:
             counts[tq] = (total, n_multi, int((q_lens == 1).sum()))
         return counts
 
-    def _context(self, lay: _Layout, n: int, nb: int, r: int, max_q: int, max_ctx: int, bound: int, all_tiles: bool = False, singles: bool = True) -> StepContext:
+    def _context(
+        self, lay: _Layout, n: int, nb: int, r: int, max_q: int, max_ctx: int, bound: int, all_tiles: bool = False, singles: bool = True, adapted: bool = False
+    ) -> StepContext:
         dev, host, o = self._dev, self._host.numpy(), lay.off
         # a captured step launches every tile its layout can hold (the list says which are live)
         tiles = {}
@@ -372,6 +383,7 @@ class ModelRunner:
             h_state_slots=host[o["state_slots"] : o["state_slots"] + nb].copy(),
             context_bound=bound,
             query_tiles=tiles,
+            adapter_ids=view("adapter_ids", n) if adapted else None,
         )
 
     # ------------------------------------------------------------------ running
@@ -382,6 +394,8 @@ class ModelRunner:
         if not items:
             return torch.empty((0, self.model.spec.vocab_size), dtype=torch.float32, device=self.rt.device)
         ops.set_pdl(self.pdl)
+        if self.rt.adapters is None and self._adapted(items):
+            raise ValueError("a step with adapters needs a runtime that keeps some (EngineConfig.adapters)")
         if self.state_slots is not None:
             fresh = self.state_slots.take_fresh()
             if fresh and self._pool is not None:
@@ -404,7 +418,7 @@ class ModelRunner:
             b_cap = next(b for b in self.graph_buckets if b >= len(items))
             n_cap = min(self.rt.max_tokens, -(-n_tok // GRAPH_TOKEN_STEP) * GRAPH_TOKEN_STEP)
             if n_rows <= b_cap and n_cap >= n_tok:
-                key = self._graph_key(items, n_cap, b_cap, decode_form=False)
+                key = (*self._graph_key(items, n_cap, b_cap, decode_form=False), self._adapted(items))
                 seen = self._graph_seen.get(key, 0) + 1
                 self._graph_seen[key] = seen
                 if seen >= self.graph_after:  # a shape that comes once is not worth a capture
@@ -414,13 +428,17 @@ class ModelRunner:
         self._ensure(lay.total)
         n, nb, r, max_q, max_ctx = self._fill(items, lay)
         self._upload(lay.total)
-        ctx = self._context(lay, n, nb, r, max_q, max_ctx, bound=0)
+        ctx = self._context(lay, n, nb, r, max_q, max_ctx, bound=0, adapted=self._adapted(items))
         before = ops.launch_count
         logits = self.model.forward(ctx)
         self.num_kernel_launches += ops.launch_count - before
         self.num_forward_passes += 1
         self.num_tokens_processed += n
         return logits[:r]
+
+    @staticmethod
+    def _adapted(items: Sequence[BatchItem]) -> bool:
+        return any(it.adapter >= 0 for it in items)
 
     _pool = None
 
@@ -444,7 +462,7 @@ class ModelRunner:
         b_cap``); else a sequence may bring any number of the tokens."""
         lay = self._layout(n_cap, b_cap, self.max_width, b_cap)
         self._ensure(lay.total)
-        key = self._graph_key(items, n_cap, b_cap, decode_form)
+        key = (*self._graph_key(items, n_cap, b_cap, decode_form), self._adapted(items))  # (once with the kernels that add adapters)
         entry = self._graphs.get(key)
         if entry is None:
             entry = self._capture(key, lay)
@@ -464,11 +482,11 @@ class ModelRunner:
         of padding only (no sequence has a query, no token has a slot), so it writes no key, no
         value and no state; the step's own arrays go to the device afterwards and the step runs
         once, as the first replay."""
-        n_cap, b_cap, reach, singles, decode_form = key
+        n_cap, b_cap, reach, singles, decode_form, adapted = key
         self._fill((), lay, padded=True, tiles=not decode_form)
         self._upload(lay.total)
         # one token per sequence: the decode form; else a sequence may bring up to all the tokens
-        ctx = self._context(lay, n_cap, b_cap, b_cap, 1 if decode_form else n_cap, reach, bound=reach, all_tiles=True, singles=singles)
+        ctx = self._context(lay, n_cap, b_cap, b_cap, 1 if decode_form else n_cap, reach, bound=reach, all_tiles=True, singles=singles, adapted=adapted)
         self.model.forward(ctx)
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()

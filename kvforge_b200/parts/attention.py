@@ -14,6 +14,7 @@ import math
 import torch
 
 from .. import ops
+from . import adapters
 from .base import CacheNeed, Mixer, PartSpec, WeightDecl, build_part, register_mixer
 from .projection import PART_ROWS, project
 
@@ -108,6 +109,8 @@ class PagedAttention(Mixer):
     convolution, the rotary kernel (or the one that also norms the heads), and the attention kernel
     that takes the shape.  The general form without a convolution and carried values also has the open form that mixers side by
     side take: ``take_input`` / ``take_output`` hand the input and output matrices over, ``mix`` computes what lies between the two products."""
+
+    qkv_bank = o_bank = None  # low-rank adapters (``parts.adapters``)
 
     def __init__(self, params, prefix=""):
         super().__init__(params, prefix)
@@ -228,6 +231,13 @@ class PagedAttention(Mixer):
             bool(self.taps) or self.dv != self.d or self.interleaved or self.qk_eps is not None or not self.plain_scores or self.value_mix is not None
         )
 
+        # low-rank adapters beside the input and the output product, where the heads lie as the checkpoint has them
+        if rt.adapters is not None and (self.d, self.dv) == (self.d_true, self.dv_true):
+            name = lambda local: self.tensor_name(local + ".weight")[: -len(".weight")]  # noqa: E731
+            widths = [self.nh * self.d, self.nkv * self.d, self.nkv * self.dv]
+            self.qkv_bank = rt.adapters.declare([name("q_proj"), name("k_proj"), name("v_proj")], widths, self.hidden)
+            self.o_bank = rt.adapters.declare([name("o_proj")], [self.hidden], self.o_dim)
+
     def _bind_position(self) -> None:
         if self.position_spec is not None and self.position is None:
             self.position = build_part("position", self.position_spec)
@@ -280,6 +290,7 @@ class PagedAttention(Mixer):
                 # decode: slices of K in parallel; the rotation kernel sums them
                 part = ops.Partials(rt.buf("attn.qkv_part", splits * n, self.qkv_dim, torch.float32, cap=PART_ROWS).view(splits, n, self.qkv_dim))
                 ops.gemm_skinny(x, self.w_qkv, part)
+                adapters.add(ctx, self.qkv_bank, x, part)
                 q = rt.buf("attn.q", n, self.q_dim)
                 ops.rope_cache_write(part, ctx.positions, self.inv_freq, slots, cache.k, cache.v, self.nh, self.nkv, self.d, ctx.block_size, rt.err, q_out=q)
                 q_stride = self.q_dim
@@ -289,6 +300,7 @@ class PagedAttention(Mixer):
                     ops.gemm_skinny(x, self.w_qkv, qkv)
                 else:
                     ops.linear(x, self.w_qkv, qkv)
+                adapters.add(ctx, self.qkv_bank, x, qkv)
                 ops.rope_cache_write(qkv, ctx.positions, self.inv_freq, slots, cache.k, cache.v, self.nh, self.nkv, self.d, ctx.block_size, rt.err)
                 q, q_stride = qkv, self.qkv_dim
         else:
@@ -299,7 +311,7 @@ class PagedAttention(Mixer):
             q_stride = self.q_dim
         out = rt.buf("attn.out", n, self.q_dim)
         self.attend(ctx, q, q_stride, out, cache)
-        return project(rt, "attn.proj", out, self.w_o, ctx)
+        return project(rt, "attn.proj", out, self.w_o, ctx, self.o_bank)
 
     def forward_general(self, ctx, x: torch.Tensor, cache):
         rt = self.rt
@@ -309,9 +321,10 @@ class PagedAttention(Mixer):
             ops.gemm_skinny(x, self.w_qkv, qkv)
         else:
             ops.linear(x, self.w_qkv, qkv)
+        adapters.add(ctx, self.qkv_bank, x, qkv)
         out = rt.buf("attn.out", n, self.o_dim)
         self.mix(ctx, qkv, cache, out)
-        return project(rt, "attn.proj", out, self.w_o, ctx)
+        return project(rt, "attn.proj", out, self.w_o, ctx, self.o_bank)
 
     inner_width = property(lambda self: self.o_dim)
 
@@ -320,10 +333,19 @@ class PagedAttention(Mixer):
         return self.general and not self.taps and self.value_mix is None
 
     def take_input(self) -> torch.Tensor:
+        self.withdraw("qkv_bank")
         w, self.w_qkv = self.w_qkv, None
         return w
 
+    def withdraw(self, *banks: str) -> None:
+        """Whoever multiplies by this part's matrices itself knows nothing of its adapters: such projections take none."""
+        for name in banks:
+            if getattr(self, name) is not None:
+                self.rt.adapters.withdraw(getattr(self, name))
+                setattr(self, name, None)
+
     def take_output(self) -> torch.Tensor:
+        self.withdraw("o_bank")
         w, self.w_o = self.w_o, None
         return w
 

@@ -7,6 +7,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
+from . import adapters
 from .base import FeedForward, WeightDecl, register_feed_forward
 from .projection import project
 
@@ -43,12 +44,26 @@ class GatedMLP(FeedForward):
         else:
             self.w_gate_up = torch.cat([gate, up], dim=0).contiguous()
         self.w_down = weights["down_proj.weight"].contiguous()
+        self.gate_up_bank = self.down_bank = None
+        if rt.adapters is not None:
+            name = lambda local: self.tensor_name(local + ".weight")[: -len(".weight")]  # noqa: E731
+            self.gate_up_bank = rt.adapters.declare([name("gate_proj"), name("up_proj")], [self.inter] * 2, self.hidden, alternating=self.interleaved)
+            self.down_bank = rt.adapters.declare([name("down_proj")], [self.hidden], self.inter)
 
     def forward(self, ctx, x: torch.Tensor):
         rt = self.rt
         n = x.shape[0]
         act = rt.buf("mlp.act", n, self.inter)
-        if self.interleaved and ops.skinny_ok(x, self.w_gate_up):
+        if self.gate_up_bank is not None and ctx.adapters is not None:
+            # adapters join gates and ups before the activation: the product as it is, then the two
+            gu = rt.buf("mlp.gate_up", n, 2 * self.inter)
+            if ops.skinny_ok(x, self.w_gate_up):
+                ops.gemm_skinny(x, self.w_gate_up, gu)
+            else:
+                ops.linear(x, self.w_gate_up, gu)
+            adapters.add(ctx, self.gate_up_bank, x, gu)
+            ops.silu_mul(gu, act, interleaved=self.interleaved)
+        elif self.interleaved and ops.skinny_ok(x, self.w_gate_up):
             ops.gemm_skinny(x, self.w_gate_up, act, mode="silu")  # a few tokens: stream the weights once
         elif self.interleaved and ops.tcgen05_ok(x, self.w_gate_up):
             # many tokens: tcgen05 tensor cores, the gate applied as the accumulator leaves tensor memory
@@ -57,7 +72,7 @@ class GatedMLP(FeedForward):
             gu = rt.buf("mlp.gate_up", n, 2 * self.inter)
             ops.linear(x, self.w_gate_up, gu)
             ops.silu_mul(gu, act, interleaved=self.interleaved)
-        return project(rt, "mlp.out", act, self.w_down, ctx)
+        return project(rt, "mlp.out", act, self.w_down, ctx, self.down_bank)
 
 
 @register_feed_forward("plain_mlp")

@@ -201,6 +201,11 @@ class DecoderModel:
                 part.position = shared_positions[key]
             local = {name: weights[part.tensor_name(name)] for name in type(part).weight_decls(part.params) if part.tensor_name(name) in weights}
             part.bind(local, rt)
+        for call in s.execution:
+            # a layer that reads another's keys multiplies by its query rows alone
+            mixer = self.blocks[call.layer].mixer_part()
+            if call.kv_from is not None and getattr(mixer, "qkv_bank", None) is not None:
+                mixer.withdraw("qkv_bank")
         # kvforge: one tensor when tied, and the embedding stands in when the head is absent
         # (src/tokenvault/model.py:157-158, src/tokenvault/model_loader.py:105-106)
         self.pass_offsets = weights[s.pass_offsets_name] if s.pass_offsets else None
@@ -224,6 +229,9 @@ class DecoderModel:
     def forward_hidden(self, ctx):
         """Runs the blocks.  Returns the float residual stream and the sum still pending."""
         rt = self.rt
+        if ctx.adapter_ids is not None:
+            ctx.adapters = rt.adapters.groups
+            ops.group_by_adapter(ctx.adapter_ids, ctx.adapters, rt.err)
         resid = rt.buf("model.resid", ctx.num_tokens, self.spec.hidden_size, torch.float32)
         self.embedding.forward(ctx, resid)
         ctx.residual = resid

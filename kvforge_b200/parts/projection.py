@@ -8,6 +8,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
+from . import adapters
 
 PART_ROWS = ops.SKINNY_MAX_M * ops.SKINNY_MAX_SPLIT  # rows of the largest set of split-K slices
 
@@ -45,11 +46,19 @@ def slices_of(rt, name: str, splits: int, n: int, width: int, ctx) -> "ops.Parti
     return ops.Partials(t)
 
 
-def project(rt, name: str, x: torch.Tensor, w: torch.Tensor, ctx=None):
+def project(rt, name: str, x: torch.Tensor, w: torch.Tensor, ctx=None, bank=None):
     """``x @ w^T`` back to the model width: the decode product (slices of K, summed by the norm
     that follows) for a few tokens, the library product otherwise.  Given the step's context, the
     library product of many bfloat16 tokens adds its result straight into the float residual
-    stream (``ctx.residual``) and ``ops.ADDED`` is returned."""
+    stream (``ctx.residual``) and ``ops.ADDED`` is returned.  ``bank``: the projection's low-rank adapters, added to whichever form the result
+    takes."""
+    y = _product(rt, name, x, w, ctx)
+    if bank is not None:
+        adapters.add(ctx, bank, x, ctx.residual[: x.shape[0]] if y is ops.ADDED else y)
+    return y
+
+
+def _product(rt, name: str, x: torch.Tensor, w: torch.Tensor, ctx):
     n, width = x.shape[0], w.shape[0]
     if ops.skinny_ok(x, w):
         splits = ops.skinny_splits(width, w.shape[1], n)
