@@ -7,8 +7,9 @@ little: a beam that goes on keeps its pages and its state slot for its first con
 are shared, and the partly filled page of every layer and the states are copied (``ops.copy_pages``, ``ops.copy_states``) into what
 the beams that end give back.
 
-The rules: of the ``2 * num_beams`` best continuations of a prompt, in order, one that ends in a stop token is a finished
-hypothesis if it is among the first ``num_beams``, and the first ``num_beams`` of the others are the next beams.  A hypothesis's score is the sum
+The rules: of a prompt's best continuations, in order, one that ends in a stop token is a finished
+hypothesis if it is among the first ``num_beams``, and the first ``num_beams`` of the others are the next beams.  (So many are looked at that all stop tokens
+of all beams leave enough, as far as the kernel's 64 candidates go; where none of them goes on, the prompt ends.)  A hypothesis's score is the sum
 of its tokens' log probabilities over its length to the power ``length_penalty``.  A prompt ends when it has ``num_beams`` finished
 hypotheses and no beam could still beat the worst of them at its present length, or at ``max_tokens`` (then the beams are hypotheses too).
 """
@@ -120,8 +121,9 @@ class BeamGroup:
 class BeamSearch:
     """Runs prompts through an engine's step function; the engine must have nothing else under way."""
 
-    def __init__(self, engine, params: BeamParams, adapter_slot: Sequence[int]) -> None:
-        self.engine, self.params = engine, params
+    def __init__(self, engine, params: BeamParams, adapter_slot: Sequence[int], stops: set[int]) -> None:
+        self.engine, self.params, self.stops = engine, params, stops
+        self.candidates = min(ops.BEAM_MAX_K, params.num_beams * (1 + max(1, len(stops))))  # a prompt
         self.core = engine.core
         self.bm, self.slots, self.pool = engine.block_manager, engine.core.state_slots, engine.kv_cache
         self.cfg = engine.config.scheduler
@@ -129,7 +131,7 @@ class BeamSearch:
         self._count = itertools.count()
         self._issued: list[str] = []  # names of the requests that hold beams
         groups = max(1, self.cfg.max_num_seqs // params.num_beams)
-        rows, k = groups * params.num_beams, 2 * params.num_beams
+        rows, k = groups * params.num_beams, self.candidates
         dev = self.core.device
         self.max_groups = groups
         self._workspace = ops.beam_workspace(rows, engine.vocab_size, k, dev)
@@ -152,8 +154,7 @@ class BeamSearch:
     # ------------------------------------------------------------------ the choice
     def _select(self, logits: torch.Tensor, scores: list[float], count: int) -> tuple[list, list, list]:
         """Per prompt of ``count``: parents, tokens and scores of its best continuations."""
-        k = 2 * self.params.num_beams
-        rows = len(scores)
+        k, rows = self.candidates, len(scores)
         self._host_scores[:rows] = torch.tensor(scores)  # (the copy before this one has been waited for: its results were read)
         self._scores[:rows].copy_(self._host_scores[:rows], non_blocking=True)
         n = count * k
@@ -252,7 +253,7 @@ class BeamSearch:
         self._move(*moved)
 
     # ------------------------------------------------------------------ all prompts
-    def run(self, prompts: Sequence[list[int]], stops: set[int]) -> list[BeamOutput]:
+    def run(self, prompts: Sequence[list[int]]) -> list[BeamOutput]:
         p, cfg, bm = self.params, self.cfg, self.bm
         groups = []
         for prompt in prompts:
@@ -264,7 +265,7 @@ class BeamSearch:
                 raise RequestRejectedError(f"a prompt of {len(prompt)} tokens exceeds max_num_batched_tokens = {cfg.max_num_batched_tokens} and prompts are not cut")
             if p.num_beams > cfg.max_num_seqs:
                 raise RequestRejectedError(f"{p.num_beams} beams are more than max_num_seqs = {cfg.max_num_seqs}")
-            group = BeamGroup(list(prompt), p, stops, min(p.max_tokens, cfg.max_model_len - len(prompt)))
+            group = BeamGroup(list(prompt), p, self.stops, min(p.max_tokens, cfg.max_model_len - len(prompt)))
             if self._reserve(group.prompt, group.limit) > bm.num_blocks:
                 raise RequestRejectedError(f"{p.num_beams} beams of {len(prompt) + group.limit} tokens can never fit the pages of the cache")
             groups.append(group)

@@ -183,14 +183,14 @@ class InferenceEngine:
         """The likeliest continuations of every prompt (``engine/beam.py``); one output per prompt, in the order given.  The engine must
         have no unfinished requests.  ``adapters``: one for all, or one per prompt."""
         if self.has_unfinished_requests():
-            raise RuntimeError("beam search needs the engine to itself: finish or abort the queued requests first")
+            raise RuntimeError("beam search needs the engine to itself: there are unfinished requests")
         params = params if params is not None else BeamParams()
         self._resolve(self._take_pending())
         slots = [self._adapter_slot(a) for a in self._per_prompt(adapters, len(prompts))]
         ids = [self._token_ids(p) for p in prompts]
         eos = getattr(self.tokenizer, "eos_token_id", None) if self.tokenizer is not None else self.core.spec.eos_token_id
         stops = set() if params.ignore_eos else {t for t in (eos, *params.stop_token_ids) if t is not None}
-        outputs = BeamSearch(self, params, slots).run(ids, stops)
+        outputs = BeamSearch(self, params, slots, stops).run(ids)
         if self.tokenizer is not None:
             for out in outputs:
                 for h in out.hypotheses:

@@ -59,7 +59,8 @@ def merged(folder, adapter):
     for key in [k for k in tensors if k.endswith("lora_A.weight")]:
         short = key[len("base_model.model.") : -len(".lora_A.weight")]
         a, b = tensors[key], tensors[key.replace("lora_A", "lora_B")]
-        plain.w[f"{short}.weight"] = plain.w[f"{short}.weight"] + scale * (b @ a)
+        own = short.removeprefix("model.") + ".weight"
+        plain.w[own] = plain.w[own] + scale * (b @ a)
     return plain
 
 
@@ -198,24 +199,30 @@ def plain_beams(plain, prompt, w, n, stops, penalty):
     """Beam search by full recomputation, in 64 bits behind the logits.  Returns (tokens, log probability) best first, and the smallest
     distance between neighbouring candidates that mattered."""
     beams, finished, gap = [([], 0.0)], [], math.inf
+    k = min(64, w * (1 + max(1, len(stops))))
     for length in range(1, n + 1):
         every = []
         for b, (tokens, lp) in enumerate(beams):
             logp = torch.log_softmax(plain.logits(prompt + tokens)[-1].double(), 0) + lp
             every += [(float(v), b, t) for t, v in enumerate(logp)]
         every.sort(key=lambda c: (-c[0], c[1], c[2]))
-        gap = min([gap, *[a[0] - b[0] for a, b in zip(every[: 2 * w], every[1 : 2 * w + 1])]])
         following = []
-        for rank, (lp, b, t) in enumerate(every[: 2 * w]):
+        for rank, (lp, b, t) in enumerate(every[:k]):
             tokens = [*beams[b][0], t]
             if t in stops:
                 if rank < w:
                     finished.append((tokens, lp))
             elif len(following) < w:
                 following.append((tokens, lp))
+                last = rank
+        # (what lies behind the last that goes on, and behind the first w, is not chosen from)
+        last = max(last, w - 1) if following else k - 1
+        gap = min([gap, *[a[0] - b[0] for a, b in zip(every[: last + 1], every[1 : last + 2])]])
         finished.sort(key=lambda h: -h[1] / len(h[0]) ** penalty)
         del finished[w:]
         beams = following
+        if not beams:
+            return finished, gap
         if len(finished) == w and beams[0][1] / length**penalty <= finished[-1][1] / len(finished[-1][0]) ** penalty:
             return finished, gap
     finished += beams
