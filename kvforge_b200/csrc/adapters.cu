@@ -53,6 +53,7 @@ struct AdapterParams {
   int alternating;
   int most;   // inner numbers of a row that shared memory holds at a time (whole sections of rank R)
   int stage;  // bytes of shared memory that columns of B and of the rows take in turn (few rows)
+  int shares; // clusters of a tile (few rows)
   int slots;  // blocks of 64 columns of k that it holds (of a warp, where there are few rows; bf16)
   int tmem;   // columns of tensor memory
 };
@@ -418,7 +419,9 @@ __device__ __forceinline__ void second_product(const AdapterParams& p, const flo
   const float* rows = b + first * p.R;
   const float* lo = inner + g * stride;
   const float* hi = lo + 8 * stride;
-  for (int r = 0; r < R16; r += 4) {
+  // (the four column groups of a warp go round the numbers from places of their own: rows of B lie a multiple of all banks apart)
+  int r = 4 * q;
+  for (int n = 0; n < R16; n += 4) {
     const float4 l = *reinterpret_cast<const float4*>(lo + r), h = *reinterpret_cast<const float4*>(hi + r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -426,6 +429,7 @@ __device__ __forceinline__ void second_product(const AdapterParams& p, const flo
       acc[0][i] = fmaf(w.w, l.w, fmaf(w.z, l.z, fmaf(w.y, l.y, fmaf(w.x, l.x, acc[0][i]))));
       acc[1][i] = fmaf(w.w, h.w, fmaf(w.z, h.z, fmaf(w.y, h.y, fmaf(w.x, h.x, acc[1][i]))));
     }
+    r = r + 4 < R16 ? r + 4 : 0;
   }
 }
 
@@ -514,7 +518,8 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
     prefetch_map(&maps.whole);
   }
   pdl_wait();
-  const int tile = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;  // (of the list: part of a tile)
+  // a tile (of the list: part of a tile) is `shares` clusters', which all make its inner numbers and share out the columns
+  const int rank = blockIdx.x % CLUSTER, tile = blockIdx.x / CLUSTER / p.shares, share = blockIdx.x / CLUSTER % p.shares * CLUSTER + rank;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
   int s, count;
   if (p.tiles) {
@@ -529,7 +534,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
   const int R = s < 0 ? 0 : p.ranks ? min(max(p.ranks[s], 0), p.R) : p.R;
   if (R == 0) {
     __syncthreads();
-    copy_rows<O>(p, rows, count, rank, CLUSTER);
+    copy_rows<O>(p, rows, count, share, CLUSTER * p.shares);
     return;
   }
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -596,8 +601,8 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
         if (sec1 == i) right = p.begin[i];
       }
     }
-    const int group = p.alternating ? 64 : 32, groups = (right - left + group - 1) / group, mine = (groups + CLUSTER - 1) / CLUSTER;
-    const int begin = rank * mine, end = min(groups, begin + mine);
+    const int group = p.alternating ? 64 : 32, groups = (right - left + group - 1) / group, mine = (groups + CLUSTER * p.shares - 1) / (CLUSTER * p.shares);
+    const int begin = share * mine, end = min(groups, begin + mine);
     const int each = max(1, (half_bytes - TILE * 128) / (group * (p.R * (int)sizeof(T) + TILE * (int)sizeof(O))));  // groups of a piece
     const auto row_stride = [&](int columns) { return (columns * (int)sizeof(O) + 63) / 128 * 128 + 64; };  // (two rows in all banks)
     const auto load = [&](int g0, int half) {  // a thread of every warp
@@ -629,12 +634,14 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
       const int c0 = left + g0 * group, columns = min(right, left + min(end, g0 + each) * group) - c0, stride = row_stride(columns);
       const char* at = reinterpret_cast<const char*>(smem) + half * half_bytes;
       const char* base = at + columns * p.R * sizeof(T);
-      for (int gi = g0 + warp; gi < min(end, g0 + each); gi += WARPS) {
-        const int from = (gi - g0) * group;  // the group's first column, from the piece's
+      // units: a group's columns of one section where they alternate, a group's where they do not
+      const int parts = p.alternating ? sec1 - sec0 : 1;
+      for (int u = warp; u < parts * (min(end, g0 + each) - g0); u += WARPS) {
+        const int from = (u >> (parts - 1)) * group;  // the group's first column, from the piece's
 #pragma unroll
         for (int i = 0; i < MAX_SECTIONS; ++i) {
           // (a group may reach over the end of a section: each takes its own columns)
-          if (i < sec0 || i >= sec1 || (!p.alternating && (c0 + from >= p.begin[i] + p.width[i] || c0 + from + 32 <= p.begin[i]))) continue;
+          if (i < sec0 || i >= sec1 || (p.alternating ? i != sec0 + (u & (parts - 1)) : c0 + from >= p.begin[i] + p.width[i] || c0 + from + 32 <= p.begin[i])) continue;
           float acc[2][8];
           second_product<SPLITS>(p, reinterpret_cast<const T*>(at) + from * p.R, columns - 1 - from, inner + (i - sec0) * R16, total, i, R16, acc);
           const int c = from + in_group(p, i, 8 * (lane & 3));
@@ -775,7 +782,9 @@ __global__ void __launch_bounds__(THREADS + 32, KEPT > 1 ? 1 : 2) adapter_outer_
   const bf16* b = reinterpret_cast<const bf16*>(p.b) + (long long)s * p.N * p.R;
   const int left = blockIdx.x * stripe * PIECE, right = min(p.N, left + stripe * PIECE);
   constexpr int ROW_BYTES = ACROSS * LIST * 128;
-  const int block = b_block(p.R), stage_bytes = ROW_BYTES + b_stage(p.R);
+  // (few rows do not mind the banks, but a warp takes some 90 cycles for every copy that it starts)
+  const bool apart = tall > 2;
+  const int block = apart ? b_block(p.R) : 16 * p.R, stage_bytes = ROW_BYTES + b_stage(p.R);
   if (warp == WARPS) {
     if (elect_one()) {
       int slot = 0, turn = 0;
@@ -795,7 +804,8 @@ __global__ void __launch_bounds__(THREADS + 32, KEPT > 1 ? 1 : 2) adapter_outer_
               for (int r = 0; r < 32 && i + r < count; r += 4) tma_gather4(to + r * 128, &maps.row, c0 + k * COLUMNS, rows[i + r], rows[i + r + 1], rows[i + r + 2], rows[i + r + 3], bar);
             }
           }
-        for (int i = 0; i < min(PIECE, right - c0) / 8; ++i) bulk_load(at + ROW_BYTES + i * block, b + (long long)(c0 + 8 * i) * p.R, 16 * p.R, bar);
+        if (!apart) bulk_load(at + ROW_BYTES, b + (long long)c0 * p.R, b_bytes, bar);
+        for (int i = 0; apart && i < min(PIECE, right - c0) / 8; ++i) bulk_load(at + ROW_BYTES + i * block, b + (long long)(c0 + 8 * i) * p.R, 16 * p.R, bar);
         if (++slot == stages) slot = 0, ++turn;
       }
     }
@@ -977,8 +987,11 @@ size_t few_smem(AdapterParams& p, int splits) {
     if (blocks > WARPS && rest + 2 * slots <= 112 * 1024) p.slots = FEW_SLOTS;
     stage = max(p.slots * slots, min(stage, (size_t)(112 * 1024 - min(rest, (size_t)48 * 1024))));
   }
-  // two groups at least (or one, and what lies between its columns) in each half
-  stage = max(stage, (size_t)2 * (64 * (p.R * sizeof(T) + TILE * sizeof(O)) + TILE * 256));
+  // in each half a group at least, and 32 columns for every warp where there is room for them (with one group of 64 columns a piece six warps
+  // of eight had nothing to do: 300 float rows of rank 64 and 28672 columns 800 us)
+  const size_t column = p.R * sizeof(T) + TILE * sizeof(O);
+  stage = max(stage, min(2 * (WARPS * 32 * column + TILE * 128), (size_t)224 * 1024 - rest));
+  stage = max(stage, 2 * (64 * column + TILE * 128));
   p.stage = (int)((stage + 2047) / 2048 * 2048);
   return rest + p.stage;
 }
@@ -997,7 +1010,7 @@ size_t many_smem(AdapterParams& p) {
 }
 static_assert(MOST <= 128 && CLUSTER * MOST * SUM_ROW * 4 + 16 * 1024 + slot_bytes(LIST, MOST) <= 220 * 1024, "one tile of the accumulator; room for a block");
 static_assert(CLUSTER * TILE * MOST * 4 + 3 * TILE * (MOST + 16) * 2 + WARPS * slot_bytes(TILE, MOST) <= 226 * 1024, "room for a block a warp");
-static_assert(CLUSTER * TILE * MOST * 4 + TILE * (MOST + 4) * 4 + 2 * (64 * (MOST * 4 + TILE * 4) + TILE * 256) + 2048 <= 226 * 1024, "... and for a float32 group a half");
+static_assert(CLUSTER * TILE * MOST * 4 + TILE * (MOST + 4) * 4 + 2 * (64 * (128 * 4 + TILE * 4) + TILE * 128) + 2048 <= 226 * 1024, "... and for a float32 group a half");
 static_assert(TILE * (MOST + 4) * 4 <= slot_bytes(TILE, MOST) && TILE * (16 + 4) * 4 <= slot_bytes(TILE, 16), "partial sums take a slot's place");
 
 // x: [n][K], one row a box and 32; A: [S sections R][K], sixteen rows a box and `most`; zeros past K
@@ -1131,10 +1144,14 @@ template <typename T, typename O, int SPLITS>
 int run_tiles(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
   static_assert(WARPS * TILE * PART * 4 <= 64 * 1024, "the partial sums take the stage's place");
   const size_t smem = few_smem<T, O>(p, SPLITS);
+  // A cluster streams all columns of B through eight SMs; where there are few tiles several clusters take shares of the columns (one row and 28672
+  // columns: 15 us with one cluster, 9 with sixteen), each of two groups or more.
+  const int groups = p.N / (p.alternating ? 64 : 32);
+  p.shares = max(1, min((smem > 112 * 1024 ? 1 : 2) * 148 / (tiles * CLUSTER), groups / (2 * CLUSTER)));
   const auto kernel = adapter_tile_kernel<T, O, SPLITS>;
   const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (rc != cudaSuccess) return (int)rc;
-  return launch(kernel, dim3(tiles * CLUSTER), dim3(THREADS), smem, st, p, maps);
+  return launch(kernel, dim3(tiles * CLUSTER * p.shares), dim3(THREADS), smem, st, p, maps);
 }
 
 }  // namespace
@@ -1185,7 +1202,7 @@ int run(AdapterParams& p, const int* ends, int wide, int max_tiles, int two, cud
   KVF_API int kvf_adapter_add_##SUF(const void* x, long long x_stride, const void* a, const void* b, const float* scales, const int* ranks, const int* ids, int n, int S,  \
                                     int sections, int R, int K, int N, int end0, int end1, int end2, int alternating, const void* base, long long base_stride, void* out,  \
                                     long long out_stride, int wide, const int* rows, const int* tiles, int max_tiles, void* inner, int two, int* err, cudaStream_t st) {   \
-    AdapterParams p{x, a, b, scales, ranks, ids, rows, tiles, (bf16*)inner, base, out, err, x_stride, base_stride, out_stride, n, S, sections, R, K, N, {}, {}, alternating, 0, 0, 0, 0}; \
+    AdapterParams p{x, a, b, scales, ranks, ids, rows, tiles, (bf16*)inner, base, out, err, x_stride, base_stride, out_stride, n, S, sections, R, K, N, {}, {}, alternating, 0, 0, 0, 0, 0}; \
     const int ends[3] = {end0, end1, end2};                                                                                                                               \
     return run<T, WIDE_SPLITS>(p, ends, wide, max_tiles, two, st);                                                                                                             \
   }

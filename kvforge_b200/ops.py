@@ -2882,7 +2882,9 @@ class AdapterBank:
 
 
 ADAPTER_DIRECT = 64  # up to so many rows the kernels group for themselves
-ADAPTER_MANY = 256  # from so many bfloat16 rows on the two products are kernels of their own
+# from so many bfloat16 rows on the two products are kernels of their own (4096 x 4096, rank 16: 512 rows 13 us in one kernel and 18 in two,
+# 2,048 rows 44 and 34; 4096 x 28672: 700 rows 56 and 42)
+ADAPTER_MANY = 640
 ADAPTER_TILE = 128  # rows of one adapter that a tile of the list has room for
 
 
