@@ -729,15 +729,14 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) adapt
   free_tensor(p, tn);
 }
 
-// ---- many rows, second kernel: a tile's rows and a stripe of columns a CTA, 64 columns at a time.  A warp of its own fetches what the pieces need (the
+// ---- many rows, second kernel: 32 rows and a stripe of columns a CTA, 256 columns at a time.  A warp of its own fetches what the pieces need (the
 // rows by TMA, 32 that follow one another a box or four gathered; the columns' rows of B are one stretch), several pieces ahead; eight
-// warps multiply, add and write 16 rows and 32 columns at a time.  What is on its way is in shared memory, not in registers: with the
-// rows in registers, fetched a group ahead, 2,048 rows of 6144 columns took 43 us in all and 1.3 TB/s here.
-constexpr int PIECE = 64;  // columns
+// warps multiply, add and write 32 columns each.  What is on its way is in shared memory, not in registers.  Pieces are wide and low because
+// rows are read and written 512 bytes at a time so: with 128 rows of 128 bytes, each in a DRAM page of its own, 2,048 rows of 6144 columns
+// went at 2.8 TB/s.
+constexpr int PIECE = 256;  // columns
+constexpr int ROWS = 32;
 constexpr int MAX_STAGES = 4;
-// eight rows of B and 64 bytes, so that the lanes of a load (rows two apart in pairs, eight apart) lie in different banks
-__host__ __device__ constexpr int b_block(int R) { return 8 * R * 2 + 64; }
-__host__ __device__ constexpr int b_stage(int R) { return (PIECE / 8 * b_block(R) + 1023) / 1024 * 1024; }  // (the next piece's swizzled rows begin at a multiple of 1,024)
 
 struct RowMaps {
   CUtensorMap run, row;  // the rows that are added to, 128 bytes a box: 32 rows, one row
@@ -746,14 +745,14 @@ struct RowMaps {
 // KEPT: sixteens of inner numbers that stay in registers from piece to piece
 template <typename O, int SPLITS, int KEPT>
 __global__ void __launch_bounds__(THREADS + 32, KEPT > 1 ? 1 : 2) adapter_outer_kernel(const __grid_constant__ AdapterParams p, const __grid_constant__ RowMaps maps, int stripe, int stages) {
-  extern __shared__ __align__(1024) char ring[];  // a piece: [128 bytes' columns][LIST rows][128 bytes], then its rows of B
-  __shared__ int rows[LIST];
-  __shared__ unsigned runs[LIST / 32];
+  extern __shared__ __align__(1024) char ring[];  // a piece: [128 bytes' columns][ROWS][128 bytes], then its rows of B
+  __shared__ int rows[ROWS];
+  __shared__ unsigned run_of;
   __shared__ __align__(8) unsigned long long filled[MAX_STAGES], empty[MAX_STAGES];
-  constexpr int ACROSS = PIECE * (int)sizeof(O) / 128;  // boxes of 128 bytes across a piece
-  constexpr int COLUMNS = 128 / (int)sizeof(O);
+  constexpr int COLUMNS = 128 / (int)sizeof(O);  // of a box
+  constexpr int ROW_BYTES = PIECE / COLUMNS * ROWS * 128;
   pdl_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, tile = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, tile = blockIdx.y / (LIST / ROWS), r0 = blockIdx.y % (LIST / ROWS) * ROWS;
   if (threadIdx.x < MAX_STAGES) {
     tc::bar_init(sm32(filled + threadIdx.x), 1);
     tc::bar_init(sm32(empty + threadIdx.x), WARPS);
@@ -764,13 +763,13 @@ __global__ void __launch_bounds__(THREADS + 32, KEPT > 1 ? 1 : 2) adapter_outer_
     prefetch_map(&maps.row);
   }
   pdl_wait();
-  const int s = p.tiles[3 * tile], first = p.tiles[3 * tile + 1], count = p.tiles[3 * tile + 2];
+  const int s = p.tiles[3 * tile], first = p.tiles[3 * tile + 1] + r0, count = min(ROWS, p.tiles[3 * tile + 2] - r0);
   if (count <= 0) return;
-  if (threadIdx.x < LIST) {
-    const int row = p.rows[first + min((int)threadIdx.x, count - 1)];  // (rows past the last are fetched and not used)
+  if (warp == 0) {
+    const int row = p.rows[first + min(lane, count - 1)];  // (rows past the last are fetched and not used)
     const bool run = __all_sync(0xffffffffu, row == __shfl_sync(0xffffffffu, row, 0) + lane);
-    rows[threadIdx.x] = row;
-    if (lane == 0) runs[threadIdx.x / 32] = run;
+    rows[lane] = row;
+    if (lane == 0) run_of = run;
   }
   __syncthreads();
   const int R = s < 0 ? 0 : p.ranks ? min(max(p.ranks[s], 0), p.R) : p.R;
@@ -778,195 +777,125 @@ __global__ void __launch_bounds__(THREADS + 32, KEPT > 1 ? 1 : 2) adapter_outer_
     if (threadIdx.x < THREADS) copy_rows<O>(p, rows, count, blockIdx.x, gridDim.x);
     return;
   }
-  const int R16 = (R + 15) & ~15, wide = p.sections * p.R, tall = (count + 15) / 16;
+  const int R16 = (R + 15) & ~15, wide = p.sections * p.R;
   const bf16* b = reinterpret_cast<const bf16*>(p.b) + (long long)s * p.N * p.R;
   const int left = blockIdx.x * stripe * PIECE, right = min(p.N, left + stripe * PIECE);
-  constexpr int ROW_BYTES = ACROSS * LIST * 128;
-  // (few rows do not mind the banks, but a warp takes some 90 cycles for every copy that it starts)
-  const bool apart = tall > 2;
-  const int block = apart ? b_block(p.R) : 16 * p.R, stage_bytes = ROW_BYTES + b_stage(p.R);
+  const int stage_bytes = ROW_BYTES + PIECE * p.R * 2;
   if (warp == WARPS) {
     if (elect_one()) {
       int slot = 0, turn = 0;
+      const int fetched = run_of ? 32 : (count + 3) / 4 * 4;
       for (int c0 = left; c0 < right; c0 += PIECE) {
         if (turn) tc::bar_wait(sm32(empty + slot), (turn - 1) & 1, p.err);
-        const uint32_t bar = sm32(filled + slot), at = sm32(ring) + slot * stage_bytes, b_bytes = min(PIECE, right - c0) * p.R * 2;
-        uint32_t bytes = b_bytes;
-        for (int i = 0; i < count; i += 32) bytes += ACROSS * (runs[i / 32] ? 32 : (min(32, count - i) + 3) / 4 * 4) * 128;
-        tc::bar_expect_tx(bar, bytes);
-        for (int i = 0; i < count; i += 32)
-#pragma unroll
-          for (int k = 0; k < ACROSS; ++k) {
-            const uint32_t to = at + (k * LIST + i) * 128;
-            if (runs[i / 32]) {
-              tc::tma_load_2d(to, &maps.run, c0 + k * COLUMNS, rows[i], bar);
-            } else {
-              for (int r = 0; r < 32 && i + r < count; r += 4) tma_gather4(to + r * 128, &maps.row, c0 + k * COLUMNS, rows[i + r], rows[i + r + 1], rows[i + r + 2], rows[i + r + 3], bar);
-            }
+        const int columns = min(PIECE, right - c0), boxes = (columns + COLUMNS - 1) / COLUMNS;
+        const uint32_t bar = sm32(filled + slot), at = sm32(ring) + slot * stage_bytes;
+        tc::bar_expect_tx(bar, boxes * fetched * 128 + columns * p.R * 2);
+        for (int k = 0; k < boxes; ++k) {
+          if (run_of) {
+            tc::tma_load_2d(at + k * ROWS * 128, &maps.run, c0 + k * COLUMNS, rows[0], bar);
+          } else {
+            for (int r = 0; r < count; r += 4) tma_gather4(at + (k * ROWS + r) * 128, &maps.row, c0 + k * COLUMNS, rows[r], rows[r + 1], rows[r + 2], rows[r + 3], bar);
           }
-        if (!apart) bulk_load(at + ROW_BYTES, b + (long long)c0 * p.R, b_bytes, bar);
-        for (int i = 0; apart && i < min(PIECE, right - c0) / 8; ++i) bulk_load(at + ROW_BYTES + i * block, b + (long long)(c0 + 8 * i) * p.R, 16 * p.R, bar);
+        }
+        bulk_load(at + ROW_BYTES, b + (long long)c0 * p.R, columns * p.R * 2, bar);
         if (++slot == stages) slot = 0, ++turn;
       }
     }
     return;
   }
-  const bf16* inner = p.inner + ((long long)tile * SPLITS * LIST + g) * wide + 4 * q;
-  // What a warp does with a whole piece of one section is the same for every piece, and is worked out here (worked out anew each time,
-  // 346 instructions for 16 x 32 numbers, the kernel was bound by them: 1.2 TB/s).  Warp w has half w % 2 of the columns (a
-  // section's, where they alternate) and rows 16 (w / 2) on, and 64 further on.
-  const int half = warp & 1, own = p.alternating ? 16 * q + 8 * half : 32 * half + 8 * q;  // the lane's first column in the piece
+  // What a warp does with a piece is the same for every piece, and is worked out here (worked out anew each time, 346 instructions for 16 x 32
+  // numbers, the kernel was bound by them).  Warp w has columns 32w .. 32w + 31, or those of section w % 2 in the 64 from
+  // 64 (w / 2) on where they alternate.
+  const int from = p.alternating ? 64 * (warp >> 1) : 32 * warp, half = warp & 1;
+  const int own = from + in_group(p, half, 8 * q);  // the lane's first column in the piece
   int w_at[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w_at[j] = (p.alternating ? (g >> 1) * 2 + half : 4 * half + (g >> 1)) * (block / 2) + (2 * j + (g & 1)) * p.R;
+  for (int j = 0; j < 4; ++j) w_at[j] = from + in_group(p, half, (g >> 1) * 8 + 2 * j + (g & 1));
   const long long split = (long long)LIST * wide;
+  const bf16* held = p.inner + ((long long)tile * SPLITS * LIST + r0 + g) * wide + 4 * q;
   O* out[2][2];
   int old_at[2][2];
-  const bf16* held[2];
   bool live[2][2];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int m = (warp >> 1) + 4 * k;
-    held[k] = inner + (long long)m * 16 * wide;
+  for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = m * 16 + 8 * h + g, byte = own * (int)sizeof(O);
+      const int r = k * 16 + 8 * h + g, byte = own * (int)sizeof(O);
       live[k][h] = r < count;
       out[k][h] = reinterpret_cast<O*>(p.out) + (live[k][h] ? rows[r] : 0) * p.out_stride + own;
-      old_at[k][h] = byte / 128 * LIST * 128 + (int)tc::sw128(r & (LIST - 1), byte % 128 / 16);
+      old_at[k][h] = byte / 128 * ROWS * 128 + (int)tc::sw128(r, byte % 128 / 16);
     }
-  }
   uint2 kept[2][KEPT][SPLITS][2];  // the first inner numbers of the section `kept_of`
   int kept_of = -1;
   int slot = 0, turn = 0;
   for (int c0 = left; c0 < right; c0 += PIECE) {
-    int sec = p.alternating ? half : 0;
-    bool whole = right - c0 >= PIECE;
-    if (!p.alternating) {
-      const int from = c0 + 32 * half;
-      int end = p.width[0];
+    tc::bar_wait(sm32(filled + slot), turn & 1, p.err);
+    const char* at = ring + slot * stage_bytes;
+    const bf16* bs = reinterpret_cast<const bf16*>(at + ROW_BYTES) + 4 * q;
+    const int columns = min(PIECE, right - c0);
 #pragma unroll
-      for (int i = 1; i < MAX_SECTIONS; ++i)
-        if (i < p.sections && from >= p.begin[i]) sec = i, end = p.begin[i] + p.width[i];
-      whole = whole && from + 32 <= end;
-    }
-    if (whole && sec != kept_of) {
-      kept_of = sec;
+    for (int i = 0; i < MAX_SECTIONS; ++i) {
+      // (32 columns may reach over the end of a section: each takes its own)
+      if (i >= p.sections || from >= columns || (p.alternating ? half != i : c0 + from >= p.begin[i] + p.width[i] || c0 + from + 32 <= p.begin[i])) continue;
+      if (i != kept_of) {
+        kept_of = i;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < KEPT; ++e)
+#pragma unroll
+            for (int t = 0; t < SPLITS; ++t) {
+              const bf16* h = held + (long long)k * 16 * wide + t * split + i * R16 + 16 * e;
+              kept[k][e][t][0] = live[k][0] && 16 * e < R16 ? *reinterpret_cast<const uint2*>(h) : make_uint2(0, 0);
+              kept[k][e][t][1] = live[k][1] && 16 * e < R16 ? *reinterpret_cast<const uint2*>(h + 8 * wide) : make_uint2(0, 0);
+            }
+      }
+      const bool mine = own < columns && (p.alternating || (c0 + own >= p.begin[i] && c0 + own < p.begin[i] + p.width[i]));
+      float acc[2][4][4];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int e = 0; e < KEPT; ++e)
-#pragma unroll
-          for (int t = 0; t < SPLITS; ++t) {
-            const bf16* h = held[k] + t * split + sec * R16 + 16 * e;
-            kept[k][e][t][0] = live[k][0] && 16 * e < R16 ? *reinterpret_cast<const uint2*>(h) : make_uint2(0, 0);
-            kept[k][e][t][1] = live[k][1] && 16 * e < R16 ? *reinterpret_cast<const uint2*>(h + 8 * wide) : make_uint2(0, 0);
-          }
-    }
-    tc::bar_wait(sm32(filled + slot), turn & 1, p.err);
-    const char* at = ring + slot * stage_bytes;
-    if (whole) {
-      const bf16* bs = reinterpret_cast<const bf16*>(at + ROW_BYTES) + 4 * q;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if ((warp >> 1) + 4 * k < tall) {
-          float acc[4][4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-          const bf16* from = held[k] + sec * R16;
-          const auto step = [&](int r, auto inner_numbers) {
-            uint2 x[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(bs + w_at[j] + r);
-#pragma unroll
-            for (int t = 0; t < SPLITS; ++t) {
-              uint2 lo, hi;
-              inner_numbers(t, lo, hi);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) mma(acc[j], lo.x, hi.x, lo.y, hi.y, x[j].x, x[j].y);
-            }
-          };
-#pragma unroll
-          for (int e = 0; e < KEPT; ++e)
-            if (16 * e < R16) step(16 * e, [&](int t, uint2& lo, uint2& hi) { lo = kept[k][e][t][0], hi = kept[k][e][t][1]; });
-          for (int r = 16 * KEPT; r < R16; r += 16)
-            step(r, [&](int t, uint2& lo, uint2& hi) {
-              lo = live[k][0] ? *reinterpret_cast<const uint2*>(from + t * split + r) : make_uint2(0, 0);
-              hi = live[k][1] ? *reinterpret_cast<const uint2*>(from + t * split + r + 8 * wide) : make_uint2(0, 0);
-            });
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (live[k][h]) {
-              uint4 old[sizeof(O) / 2];
-#pragma unroll
-              for (int e = 0; e < (int)sizeof(O) / 2; ++e) old[e] = *reinterpret_cast<const uint4*>(at + (old_at[k][h] ^ (16 * e)));  // (the next sixteen bytes of a swizzled row)
-              const float v[8] = {acc[0][2 * h], acc[0][2 * h + 1], acc[1][2 * h], acc[1][2 * h + 1], acc[2][2 * h], acc[2][2 * h + 1], acc[3][2 * h], acc[3][2 * h + 1]};
-              add_eight(old, out[k][h] + c0, v);
-            }
-          }
-        }
-      }
-      __syncwarp();
-      if (lane == 0) tc::bar_arrive(sm32(empty + slot));
-      if (++slot == stages) slot = 0, ++turn;
-      continue;
-    }
-    // a piece that the row ends in, or with the end of a section in it
-    const bf16* bs = reinterpret_cast<const bf16*>(at + ROW_BYTES) + 4 * q;
-    const int columns = min(PIECE, right - c0);
-    for (int u = warp; u < 2 * tall; u += WARPS) {
-      const int m = u >> 1;  // 16 rows; 32 columns, or those of a section where they alternate
-      const bool low = m * 16 + g < count, high = m * 16 + g + 8 < count;
-      const int from = p.alternating ? 0 : 32 * half;
-#pragma unroll
-      for (int i = 0; i < MAX_SECTIONS; ++i) {
-        // (32 columns may reach over the end of a section: each takes its own)
-        if (i >= p.sections || from >= columns || (p.alternating ? half != i : c0 + from >= p.begin[i] + p.width[i] || c0 + from + 32 <= p.begin[i])) continue;
-        // column 2q + e of the j-th of four tensor-core tiles is column 8q + 2j + e of the 32, so that a lane's eight results lie side by side
-        const bf16* w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = min(from + in_group(p, i, (g >> 1) * 8 + 2 * j + (g & 1)), columns - 1);  // (columns past the last are not written)
-          w[j] = bs + (c >> 3) * (block / 2) + (c & 7) * p.R;
-        }
-        float acc[4][4];
-#pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) acc[j][k] = 0.f;
-        const bf16* held = inner + (long long)m * 16 * wide + i * R16;
-        for (int r = 0; r < R16; r += 16) {
-          uint2 x[4];
+          for (int e = 0; e < 4; ++e) acc[k][j][e] = 0.f;
+      const auto step = [&](int r, auto inner_numbers) {
+        uint2 x[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(w[j] + r);
+        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint2*>(bs + min(w_at[j], columns - 1) * p.R + r);  // (columns past the last are not written)
 #pragma unroll
-          for (int k = 0; k < SPLITS; ++k) {
-            const bf16* h = held + (long long)k * LIST * wide + r;
-            const uint2 lo = low ? *reinterpret_cast<const uint2*>(h) : make_uint2(0, 0), hi = high ? *reinterpret_cast<const uint2*>(h + 8 * wide) : make_uint2(0, 0);
+        for (int k = 0; k < 2; ++k) {
+          if (k && count <= 16) continue;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mma(acc[j], lo.x, hi.x, lo.y, hi.y, x[j].x, x[j].y);
+          for (int t = 0; t < SPLITS; ++t) {
+            uint2 lo, hi;
+            inner_numbers(k, t, lo, hi);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma(acc[k][j], lo.x, hi.x, lo.y, hi.y, x[j].x, x[j].y);
           }
         }
-        const int c = from + in_group(p, i, 8 * q);
-        const bool mine = c < columns && (p.alternating || (c0 + c >= p.begin[i] && c0 + c < p.begin[i] + p.width[i]));
+      };
+#pragma unroll
+      for (int e = 0; e < KEPT; ++e)
+        if (16 * e < R16) step(16 * e, [&](int k, int t, uint2& lo, uint2& hi) { lo = kept[k][e][t][0], hi = kept[k][e][t][1]; });
+      for (int r = 16 * KEPT; r < R16; r += 16)
+        step(r, [&](int k, int t, uint2& lo, uint2& hi) {
+          const bf16* h = held + (long long)k * 16 * wide + t * split + i * R16 + r;
+          lo = live[k][0] ? *reinterpret_cast<const uint2*>(h) : make_uint2(0, 0);
+          hi = live[k][1] ? *reinterpret_cast<const uint2*>(h + 8 * wide) : make_uint2(0, 0);
+        });
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int r = m * 16 + g + 8 * h;
-          if (mine && r < count) {
+          if (mine && live[k][h]) {
             uint4 old[sizeof(O) / 2];
 #pragma unroll
-            for (int k = 0; k < (int)sizeof(O) / 2; ++k) {
-              const int byte = c * (int)sizeof(O) + 16 * k;
-              old[k] = *reinterpret_cast<const uint4*>(at + byte / 128 * LIST * 128 + tc::sw128(r, byte % 128 / 16));
-            }
-            const float v[8] = {acc[0][2 * h], acc[0][2 * h + 1], acc[1][2 * h], acc[1][2 * h + 1], acc[2][2 * h], acc[2][2 * h + 1], acc[3][2 * h], acc[3][2 * h + 1]};
-            add_eight(old, reinterpret_cast<O*>(p.out) + rows[r] * p.out_stride + c0 + c, v);
+            for (int e = 0; e < (int)sizeof(O) / 2; ++e) old[e] = *reinterpret_cast<const uint4*>(at + (old_at[k][h] ^ (16 * e)));  // (the next sixteen bytes of a swizzled row)
+            const float v[8] = {acc[k][0][2 * h], acc[k][0][2 * h + 1], acc[k][1][2 * h], acc[k][1][2 * h + 1], acc[k][2][2 * h], acc[k][2][2 * h + 1], acc[k][3][2 * h], acc[k][3][2 * h + 1]};
+            add_eight(old, out[k][h] + c0, v);
           }
         }
-        __syncwarp();  // (the next products take the whole warp)
-      }
+      __syncwarp();  // (the next products take the whole warp)
     }
     __syncwarp();
     if (lane == 0) tc::bar_arrive(sm32(empty + slot));
@@ -1042,9 +971,9 @@ int run_wide(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
       return (int)cudaErrorInvalidValue;
   }
   const bool few_ranks = p.R <= 16;
-  const size_t one = many_smem(p), stage = (size_t)PIECE * sizeof(O) * LIST + (size_t)b_stage(p.R);
+  const size_t one = many_smem(p), stage = (size_t)PIECE * sizeof(O) * ROWS + (size_t)PIECE * p.R * 2;
   const int places = few_ranks ? 2 : 1;  // CTAs an SM: more inner numbers in registers leave room for one
-  const int stages = max(2, min(MAX_STAGES, (int)(220 * 1024 / places / stage)));
+  const int stages = min(MAX_STAGES, (int)(220 * 1024 / places / stage));  // (of 96 KB at the most: two at least)
   const auto inner = adapter_inner_kernel<SPLITS>;
   const auto outer = few_ranks ? adapter_outer_kernel<O, SPLITS, 1> : adapter_outer_kernel<O, SPLITS, 4>;
   cudaError_t rc = cudaFuncSetAttribute(inner, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one);
@@ -1053,9 +982,9 @@ int run_wide(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
   const int r = launch(inner, dim3(tiles * CLUSTER), dim3(THREADS), one, st, p, maps);
   if (r) return r;
   // pieces of a CTA: as many as leave a CTA for every place there is
-  const int pieces = (p.N + PIECE - 1) / PIECE, full = (p.n + LIST - 1) / LIST;
+  const int pieces = (p.N + PIECE - 1) / PIECE, full = (p.n + ROWS - 1) / ROWS;
   const int stripe = max(1, min(pieces, (int)(((long long)pieces * full + places * 148 - 1) / (places * 148))));
-  return launch(outer, dim3((pieces + stripe - 1) / stripe, tiles), dim3(THREADS + 32), stages * stage, st, p, base, stripe, stages);
+  return launch(outer, dim3((pieces + stripe - 1) / stripe, tiles * (LIST / ROWS)), dim3(THREADS + 32), stages * stage, st, p, base, stripe, stages);
 }
 
 // ---- the rows of a step by adapter: one CTA.  Rows without an adapter come last.  The rows of an adapter keep their order within a
