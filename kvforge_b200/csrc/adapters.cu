@@ -1127,13 +1127,15 @@ int run(AdapterParams& p, const int* ends, int wide, int max_tiles, int two, cud
 
 }  // namespace
 
+// A bank as the host keeps it for all calls: A, B, scales, ranks (or null), adapters, sections, R, K, N, the first three sections' ends,
+// whether they alternate; 64 bits each.
 #define KVF_ADAPTER_API(SUF, T, WIDE_SPLITS)                                                                                                                              \
-  KVF_API int kvf_adapter_add_##SUF(const void* x, long long x_stride, const void* a, const void* b, const float* scales, const int* ranks, const int* ids, int n, int S,  \
-                                    int sections, int R, int K, int N, int end0, int end1, int end2, int alternating, const void* base, long long base_stride, void* out,  \
+  KVF_API int kvf_adapter_add_##SUF(const void* x, long long x_stride, const long long* bank, const int* ids, int n, const void* base, long long base_stride, void* out,  \
                                     long long out_stride, int wide, const int* rows, const int* tiles, int max_tiles, void* inner, int two, int* err, cudaStream_t st) {   \
-    AdapterParams p{x, a, b, scales, ranks, ids, rows, tiles, (bf16*)inner, base, out, err, x_stride, base_stride, out_stride, n, S, sections, R, K, N, {}, {}, alternating, 0, 0, 0, 0, 0}; \
-    const int ends[3] = {end0, end1, end2};                                                                                                                               \
-    return run<T, WIDE_SPLITS>(p, ends, wide, max_tiles, two, st);                                                                                                             \
+    AdapterParams p{x, (const void*)bank[0], (const void*)bank[1], (const float*)bank[2], (const int*)bank[3], ids, rows, tiles, (bf16*)inner, base, out, err, x_stride,    \
+                    base_stride, out_stride, n, (int)bank[4], (int)bank[5], (int)bank[6], (int)bank[7], (int)bank[8], {}, {}, (int)bank[12], 0, 0, 0, 0, 0};               \
+    const int ends[3] = {(int)bank[9], (int)bank[10], (int)bank[11]};                                                                                                      \
+    return run<T, WIDE_SPLITS>(p, ends, wide, max_tiles, two, st);                                                                                                        \
   }
 KVF_ADAPTER_API(f32, float, 1)
 KVF_ADAPTER_API(bf16, bf16, 3)

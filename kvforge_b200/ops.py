@@ -99,7 +99,7 @@ _SIGNATURES = {
     "kvf_copy_states": "pilppiiip",
     "kvf_beams_set_pdl": "i",
     # library "adapters"
-    "kvf_adapter_add_{s}": "plppppp" + "i" * 6 + "i" * 4 + "plplippipipp",
+    "kvf_adapter_add_{s}": "plppiplplippipipp",
     "kvf_adapter_group": "piiiipppp",
     "kvf_adapters_set_pdl": "i",
 }
@@ -2704,12 +2704,15 @@ def _here(*tensors: torch.Tensor | None) -> None:
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        device = t.get_device()
+        if device == here:
+            continue
+        if device < 0:
             raise RuntimeError("every operand must be a CUDA tensor (this engine has no CPU path)")
         if here is None:
             here = torch.cuda.current_device()
-        if t.get_device() != here:
-            raise ValueError(f"an operand lives on device {t.get_device()}, the current device is {here}")
+        if device != here:
+            raise ValueError(f"an operand lives on device {device}, the current device is {here}")
 
 
 BEAM_MAX_K = 64  # candidates a prompt
@@ -2780,7 +2783,7 @@ def copy_pages(k: torch.Tensor, v: torch.Tensor | None, src: torch.Tensor, dst: 
     n = _pairs(src, dst, "copy_pages")
     if tokens is not None and (tokens.dtype != torch.int32 or not tokens.is_contiguous() or tokens.numel() != n):
         raise ValueError("copy_pages: tokens are contiguous int32, one count a pair")
-    if k.dim() != 5 or not k.is_contiguous() or (v is not None and (v.shape[:4] != k.shape[:4] or v.dim() != 5 or v.dtype != k.dtype or not v.is_contiguous())):
+    if k.dim() != 5 or not k.is_contiguous() or (v is not None and (v.dim() != 5 or v.shape[:4] != k.shape[:4] or v.dtype != k.dtype or not v.is_contiguous())):
         raise ValueError("copy_pages: keys and values are contiguous [entries, pages, heads, page size, head] of one type")
     entries, blocks, heads, bs, d = k.shape
     size = k.element_size()
@@ -2879,6 +2882,12 @@ class AdapterBank:
         self.a, self.b, self.scales, self.ranks = a, b, scales, ranks
         self.ends, self.alternating = ends, bool(alternating)
         self.size, self.sections, self.rank, self.k, self.n = s, sections, r, k, n
+        # what every call hands to the launcher
+        self.dtype, self.suffix = a.dtype, _suffix(a.dtype)
+        e = (*self.ends, n, n)
+        self._words = (ctypes.c_longlong * 13)(_ptr(a), _ptr(b), _ptr(scales), _ptr(ranks) or 0, s, sections, r, k, n, e[0], e[1], e[2], int(self.alternating))
+        self._address = ctypes.addressof(self._words)
+        self._step = 16 // a.element_size()  # rows of x begin at multiples of 16 bytes
 
 
 ADAPTER_DIRECT = 64  # up to so many rows the kernels group for themselves
@@ -2930,35 +2939,36 @@ def group_by_adapter(ids: torch.Tensor, groups: AdapterGroups, err: torch.Tensor
 def adapter_add(x: torch.Tensor, bank: AdapterBank, groups: AdapterGroups, out: torch.Tensor, base: torch.Tensor | None = None) -> None:
     """``out[n] = base[n] + scales[s] * b[s] (a[s] x[n])`` with the adapter ``s`` of row ``n`` (``group_by_adapter``), and ``base[n]`` where that is
     -1.  ``x [N, K]`` in the bank's type; ``out`` and ``base`` ``[N, width]`` in it or in float32.  ``base=None``: ``out`` is added to."""
-    s = _suffix(bank.a.dtype)
     n, k = x.shape
-    if x.dtype != bank.a.dtype or k != bank.k or x.stride(1) != 1 or (x.stride(0) * x.element_size()) % 16 or x.data_ptr() % 16:
+    dtype, ld = bank.dtype, x.stride()
+    if x.dtype != dtype or k != bank.k or ld[1] != 1 or ld[0] % bank._step or x.data_ptr() % 16:
         raise ValueError("adapter_add: x must be [N, K] of the bank's type and width, its rows at multiples of 16 bytes")
     if groups.n != n or groups.ids is None or groups.num_adapters != bank.size:
         raise ValueError("adapter_add: the groups are not those of these rows and this bank")
-    base = out if base is None else base
-    for t, what in ((out, "out"), (base, "base")):
-        if t.dtype not in (bank.a.dtype, torch.float32) or t.dtype != out.dtype or tuple(t.shape) != (n, bank.n):
-            raise ValueError(f"adapter_add: {what} must be [N, {bank.n}] of the bank's type or float32")
-        if t.stride(1) != 1 or (t.stride(0) * t.element_size()) % 16 or t.data_ptr() % 16:
-            raise ValueError(f"adapter_add: {what} needs unit inner stride and rows at multiples of 16 bytes")
-    if base is not out and base.data_ptr() == out.data_ptr() and base.stride(0) != out.stride(0):
-        raise ValueError("adapter_add: base and out overlap")
+    wide, lo = out.dtype == torch.float32, out.stride()
+    step = 4 if wide else 8
+    if (not wide and out.dtype != dtype) or out.shape != (n, bank.n) or lo[1] != 1 or lo[0] % step or out.data_ptr() % 16:
+        raise ValueError(f"adapter_add: out must be [N, {bank.n}] of the bank's type or float32, its rows at multiples of 16 bytes")
+    if base is None:
+        base, lb = out, lo
+    else:
+        lb = base.stride()
+        if base.dtype != out.dtype or base.shape != (n, bank.n) or lb[1] != 1 or lb[0] % step or base.data_ptr() % 16:
+            raise ValueError("adapter_add: base must be as out, its rows at multiples of 16 bytes")
+        if base.data_ptr() == out.data_ptr() and lb[0] != lo[0] and n > 1:
+            raise ValueError("adapter_add: base and out overlap")
+    if bank.sections * bank.rank > groups.max_rows:
+        raise ValueError(f"adapter_add: the groups were made for {groups.max_rows} rows of a bank's adapters, this bank's have {bank.sections * bank.rank}")
     _here(x, bank.a, out, base, groups.ids)
     if n == 0:
         return
-    if bank.sections * bank.rank > groups.max_rows:
-        raise ValueError(f"adapter_add: the groups were made for {groups.max_rows} rows of a bank's adapters, this bank's have {bank.sections * bank.rank}")
-    two = n >= ADAPTER_MANY and s == "bf16"
-    ends = (*bank.ends, bank.n, bank.n)
-    listed = n > ADAPTER_DIRECT
-    name = f"kvf_adapter_add_{s}"
+    two, listed = n >= ADAPTER_MANY and dtype == torch.bfloat16, n > ADAPTER_DIRECT
+    name = "kvf_adapter_add_bf16" if dtype == torch.bfloat16 else "kvf_adapter_add_f32"
     _check(
         _fn(name, "adapters")(
-            _ptr(x), x.stride(0), _ptr(bank.a), _ptr(bank.b), _ptr(bank.scales), _ptr(bank.ranks), _ptr(groups.ids), n, bank.size, bank.sections, bank.rank, k, bank.n,
-            ends[0], ends[1], ends[2], int(bank.alternating), _ptr(base), base.stride(0), _ptr(out), out.stride(0), int(out.dtype == torch.float32),
-            _ptr(groups.rows), _ptr(groups.tiles) if listed else None, groups.max_tiles(n) if listed else 0, _ptr(groups.inner) if two else None,
-            int(two), _ptr(groups.err), _stream(),
+            x.data_ptr(), ld[0], bank._address, groups.ids.data_ptr(), n, base.data_ptr(), lb[0], out.data_ptr(), lo[0], wide,
+            groups.rows.data_ptr() if listed else None, groups.tiles.data_ptr() if listed else None, groups.max_tiles(n) if listed else 0,
+            groups.inner.data_ptr() if two else None, two, _ptr(groups.err), _stream(),
         ),
         name, 2 if two else 1,
     )  # fmt: skip
