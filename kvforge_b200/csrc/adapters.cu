@@ -3,18 +3,18 @@
 // and base[n] where s is -1.  A section is one of the matrices that are stacked in the projection (queries, keys, values);
 // of gates and ups that alternate in blocks of 8 columns the sections alternate too.
 //
-// bfloat16, the first product: on the tcgen05 tensor cores, by a cluster of eight CTAs that share out k in blocks of 64 columns; the adapter's
-// rows of A are the 128 lanes of the accumulator, the tile's rows its columns, so that 16 rows cost as little as a product of 128 x 16 and no
-// register holds what is on its way (A comes by TMA, the rows of x gathered by TMA four at a time, several blocks ahead).  Rows of A past the
-// adapter's are whatever lies there in shared memory: their lanes are not read.  Every CTA's sums go to the CTAs that need them through shared memory and are added in
-// one order.
-// The second product has 16 to 128 k and thousands of columns, each read and written once: mma.sync with operands straight from
-// memory (a lane takes eight bytes of a row of B; which of its k come first is its own affair as long as the inner numbers agree), bound
-// by the rows that are read and written.  The numbers between the products are sums in 32 bits and are multiplied as two bfloat16 numbers
-// (2^-17 of each is lost beside a result that is rounded to 2^-8), or as three where the result is float.  float32 stays on the FP32 pipes.
+// What bounds it is bytes (about a rank's flops a byte of x and of the rows) and, for few rows, latency.  The numbers between the two
+// products ("inner" numbers) are sums in 32 bits; bfloat16 multiplies them as two bfloat16 numbers (2^-17 of each is lost beside a result that
+// is rounded to 2^-8), or as three where the result is float.  float32 stays on the FP32 pipes.  A row's sums come in one order whatever
+// else is in the step: partial sums of k meet in shared memory and are added warp by warp and CTA by CTA.
 //
-// Few rows (and float32): one launch, a cluster makes 16 rows' inner numbers in all its CTAs and then each CTA an eighth of the columns.
-// Many rows: two launches.  A cluster makes 128 rows' inner numbers; then 64 rows and some hundred columns are a CTA.
+// Few rows (and float32), one launch (`adapter_tile_kernel`): 16 rows of one adapter go to a cluster of eight CTAs.  Each warp multiplies blocks of
+// 64 columns of k of its own (mma.sync; A comes by TMA, the rows of x by TMA, gathered, four at a time); the CTAs' sums go to all eight through
+// their shared memory; then each CTA adds its share of the columns, B and the rows that are added to coming by bulk copies, a piece
+// ahead.  Where there are few tiles several clusters make the same inner numbers and share out the columns.
+// Many rows, two launches: `adapter_inner_kernel`, 128 rows by a cluster (tcgen05: the adapter's rows of A are the lanes of the accumulator, the
+// tile's rows its columns; rows of A past the adapter's are whatever lies there in shared memory, and their lanes are not read), and
+// `adapter_outer_kernel`, 32 rows and some hundred columns a CTA.
 //
 // Which rows make a tile: up to 64 rows every cluster finds out for itself; for more a kernel of one CTA sorts the rows once a step.
 #include "tcgen05.cuh"
@@ -504,6 +504,9 @@ __device__ __forceinline__ int own_rows(const AdapterParams& p, int t, int* rows
   return count;
 }
 
+// Measured (replayed launches, inputs from three states in turn): eight rows with adapters of their own, rank 16, 4096 -> 6144 9.3 us for 5.0
+// MB; 64 rows on 20 adapters, rank 32, 8192 -> 2048 in float 10.9 us for 15 MB; one row, 4096 -> 28672 8.4 us; 512 rows of one adapter, 4096 ->
+// 4096 13 us for 13 MB.  Of the 9.3 us some 1 goes to the ids, 2 to x and A, 2 to the sums and the cluster's barrier, 2 to B and the rows.
 // T: type of x, A and B; O: of base and out
 template <typename T, typename O, int SPLITS>
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) adapter_tile_kernel(const __grid_constant__ AdapterParams p, const __grid_constant__ Maps maps) {
@@ -665,7 +668,9 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
   }
 }
 
-// ---- many rows, first kernel: the inner numbers of 128 rows by a cluster, of which CTA c keeps rows 16c .. 16c + 15
+// ---- many rows, first kernel: the inner numbers of 128 rows by a cluster, of which CTA c keeps rows 16c .. 16c + 15.  2,048 rows of 4096 columns and
+// 48 rows of A (17 MB) 11 us behind the kernel that sorts them (4 us): the loads take 3, the eight products of a block some 0.3 each behind the
+// last of them, the sums and the cluster's barrier 3.
 template <int SPLITS>
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) adapter_inner_kernel(const __grid_constant__ AdapterParams p, const __grid_constant__ Maps maps) {
   extern __shared__ __align__(1024) float smem[];  // the ring of blocks, then the sums
@@ -731,9 +736,9 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) adapt
 
 // ---- many rows, second kernel: 32 rows and a stripe of columns a CTA, 256 columns at a time.  A warp of its own fetches what the pieces need (the
 // rows by TMA, 32 that follow one another a box or four gathered; the columns' rows of B are one stretch), several pieces ahead; eight
-// warps multiply, add and write 32 columns each.  What is on its way is in shared memory, not in registers.  Pieces are wide and low because
-// rows are read and written 512 bytes at a time so: with 128 rows of 128 bytes, each in a DRAM page of its own, 2,048 rows of 6144 columns
-// went at 2.8 TB/s.
+// warps multiply, add and write 32 columns each.  What is on its way is in shared memory, not in registers.  2,048 rows of 6144 columns, rank 16 (50
+// MB) 20 us; 1,057 rows on 24 adapters of rank 64, 28672 columns (238 MB) some 115 us of 161, of which the products are 32 and the writes 18.
+// Pieces of 128 rows and 64 columns, whose warps stand idle where an adapter has one row, took 145 us there (and 18 for the first).
 constexpr int PIECE = 256;  // columns
 constexpr int ROWS = 32;
 constexpr int MAX_STAGES = 4;
@@ -1118,7 +1123,7 @@ int run(AdapterParams& p, const int* ends, int wide, int max_tiles, int two, cud
   if constexpr (sizeof(T) == 2) {
     const int rc = make_maps(p, maps);
     if (rc) return rc;
-    if (two && p.tiles && p.inner && max_tiles <= 65535) return wide ? run_wide<float, 3>(p, maps, max_tiles, st) : run_wide<bf16, 2>(p, maps, max_tiles, st);
+    if (two && p.tiles && p.inner && max_tiles * (LIST / ROWS) <= 65535) return wide ? run_wide<float, 3>(p, maps, max_tiles, st) : run_wide<bf16, 2>(p, maps, max_tiles, st);
   }
   const int tiles = p.tiles ? max_tiles * (LIST / TILE) : p.n;
   if (wide) return run_tiles<T, float, WIDE_SPLITS>(p, maps, tiles, st);

@@ -9,6 +9,8 @@
 // The K highest are found without a sort: every warp's m-th highest thread maximum (m = K / 8 rounded up) has at least K numbers of the CTA
 // at or above the least of the eight, a bound that rises as the walk goes on and that a few dozen numbers of a stretch pass; those are
 // gathered, and each counts the ones above it.  Where too many pass (rows of one value), the K highest are taken one after another.
+// Measured: 512 rows of 128,256 logits (64 prompts of eight beams, K = 16) 57 us, 4.6 TB/s, bound by the instructions of the walk (some 13 a
+// logit and warp); four rows 9.4 us, of which the walk is 1.5, the choice 1, the ticket 1, the join 3 and the launch the rest.
 // Order is decided in 64 bits (a logit with its place; a score in double with its place), so equal numbers never depend on which
 // thread comes first; sums of sixteen exponentials are in float, all that joins them is in double and in one order.
 #include "common.cuh"

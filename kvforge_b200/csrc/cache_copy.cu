@@ -2,6 +2,8 @@
 //
 // A copy is a pair (source, target); no target is a source or the target of another pair, so copies need no order.  A pair with an
 // index outside the pool copies nothing.
+// Bound by bytes: 192 pages of 32 layers of 8 heads of 128 (428 MB read and written) 67 us, 6.4 TB/s; 20 states of 13.8 MB 66 us (a
+// source that two targets share is read once).
 #include "common.cuh"
 
 using namespace kvf;

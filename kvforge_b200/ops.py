@@ -2938,22 +2938,28 @@ def group_by_adapter(ids: torch.Tensor, groups: AdapterGroups, err: torch.Tensor
 
 def adapter_add(x: torch.Tensor, bank: AdapterBank, groups: AdapterGroups, out: torch.Tensor, base: torch.Tensor | None = None) -> None:
     """``out[n] = base[n] + scales[s] * b[s] (a[s] x[n])`` with the adapter ``s`` of row ``n`` (``group_by_adapter``), and ``base[n]`` where that is
-    -1.  ``x [N, K]`` in the bank's type; ``out`` and ``base`` ``[N, width]`` in it or in float32.  ``base=None``: ``out`` is added to."""
+    -1.  ``x [N, K]`` in the bank's type; ``out`` and ``base`` ``[N, width]`` in it or in float32.  ``base=None``: ``out`` is added to; else the
+    two do not overlap, nor does ``out`` with ``x``.  Sums are in 32 bits, rounded once to the type of ``out``; a row's result does not depend on what
+    else is in the step but through the kernel that its number of rows selects."""
     n, k = x.shape
     dtype, ld = bank.dtype, x.stride()
-    if x.dtype != dtype or k != bank.k or ld[1] != 1 or ld[0] % bank._step or x.data_ptr() % 16:
+    if n <= 1:  # (how far it is to a row that there is not says nothing)
+        ld = (k, ld[1] if k > 1 else 1)
+    if x.dtype != dtype or k != bank.k or ld[1] != 1 or ld[0] < k or ld[0] % bank._step or x.data_ptr() % 16:
         raise ValueError("adapter_add: x must be [N, K] of the bank's type and width, its rows at multiples of 16 bytes")
     if groups.n != n or groups.ids is None or groups.num_adapters != bank.size:
         raise ValueError("adapter_add: the groups are not those of these rows and this bank")
     wide, lo = out.dtype == torch.float32, out.stride()
-    step = 4 if wide else 8
-    if (not wide and out.dtype != dtype) or out.shape != (n, bank.n) or lo[1] != 1 or lo[0] % step or out.data_ptr() % 16:
+    step, few = 4 if wide else 8, n <= 1
+    if few:
+        lo = (bank.n, lo[1])
+    if (not wide and out.dtype != dtype) or out.shape != (n, bank.n) or lo[1] != 1 or lo[0] < bank.n or lo[0] % step or out.data_ptr() % 16:
         raise ValueError(f"adapter_add: out must be [N, {bank.n}] of the bank's type or float32, its rows at multiples of 16 bytes")
     if base is None:
         base, lb = out, lo
     else:
-        lb = base.stride()
-        if base.dtype != out.dtype or base.shape != (n, bank.n) or lb[1] != 1 or lb[0] % step or base.data_ptr() % 16:
+        lb = (bank.n, base.stride(1)) if few else base.stride()
+        if base.dtype != out.dtype or base.shape != (n, bank.n) or lb[1] != 1 or lb[0] < bank.n or lb[0] % step or base.data_ptr() % 16:
             raise ValueError("adapter_add: base must be as out, its rows at multiples of 16 bytes")
         if base.data_ptr() == out.data_ptr() and lb[0] != lo[0] and n > 1:
             raise ValueError("adapter_add: base and out overlap")
