@@ -975,7 +975,9 @@ int run_wide(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return (int)cudaErrorInvalidValue;
   }
-  const bool few_ranks = p.R <= 16;
+  // (2,048 float rows on eight adapters of rank 32, 4096 columns: 42 us so, 63 with more numbers in registers and one CTA an SM; 2,048 of rank 64: 91
+  // and 81)
+  const bool few_ranks = p.R <= 32;
   const size_t one = many_smem(p), stage = (size_t)PIECE * sizeof(O) * ROWS + (size_t)PIECE * p.R * 2;
   const int places = few_ranks ? 2 : 1;  // CTAs an SM: more inner numbers in registers leave room for one
   const int stages = min(MAX_STAGES, (int)(220 * 1024 / places / stage));  // (of 96 KB at the most: two at least)
