@@ -14,6 +14,7 @@
 // ahead.  Where there are few tiles several clusters make the same inner numbers and share out the columns.
 // Many rows, two launches: `adapter_inner_kernel`, 128 rows by a cluster (tcgen05: the adapter's rows of A are the lanes of the accumulator, the
 // tile's rows its columns; rows of A past the adapter's are whatever lies there in shared memory, and their lanes are not read), and
+// `adapter_outer_tensor_kernel`, 128 rows and a stripe of columns a CTA on tcgen05, or, where that has no room for the inner numbers of a tile,
 // `adapter_outer_kernel`, 32 rows and some hundred columns a CTA.
 //
 // Which rows make a tile: up to 64 rows every cluster finds out for itself; for more a kernel of one CTA sorts the rows once a step.
@@ -240,9 +241,10 @@ struct Tensor {
 
 // Many rows: this CTA's share of a[total rows][k] x[128 rows][k], sent to where it is needed: CTA c of the cluster gets the sums of rows
 // 16c .. 16c + 15 of x, in `sums[rank][t][SUM_ROW]`.  a0: the first of the sections' rows of A among all adapters'; rows:
-// of x, each valid; runs: bit i, rows 32i .. 32i + 31 follow one another in x.  Blocks are the cluster's in turn: block j of the CTA is block
+// of x, `count`, to the next multiple of four each valid; runs: bit i, rows 32i .. 32i + 31 follow one another in x.  What lies where no rows are fetched
+// reaches only the sums of those.  Blocks are the cluster's in turn: block j of the CTA is block
 // rank + 8 j of k.  Warp 0 multiplies; a slot is filled by a thread of a warp of its own (a warp takes some 90 cycles for each copy that it starts).
-__device__ __forceinline__ void first_product(const AdapterParams& p, const Maps& maps, int a0, const int* rows, unsigned runs, int total, int R16, int rank, Tensor& tn, float* sums) {
+__device__ __forceinline__ void first_product(const AdapterParams& p, const Maps& maps, int a0, const int* rows, unsigned runs, int count, int total, int R16, int rank, Tensor& tn, float* sums) {
   constexpr int NR = LIST;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int every = (p.K + BLOCK_K - 1) / BLOCK_K, blocks = (every - rank + CLUSTER - 1) / CLUSTER;  // (none for some where K is short)
@@ -254,13 +256,14 @@ __device__ __forceinline__ void first_product(const AdapterParams& p, const Maps
     // (a parity tells only two neighbouring phases apart).
     // Where all rows follow one another a block is a few copies, and one warp starts them block after block: the first block is there first.
     const bool alone = runs == (1u << LIST / 32) - 1;
+    const int fetched = (count + 3) / 4 * 4;
     if (warp <= (alone ? 1 : p.slots) && elect_one()) {
       const int begin = tn.block % p.slots, own = warp - 1;
       for (int j = alone ? 0 : own - begin + (own < begin ? p.slots : 0); j < blocks; j += alone ? 1 : p.slots) {
         const int turn = (tn.block + j) / p.slots, slot = (tn.block + j) % p.slots;
         if (turn) tc::bar_wait(done + 8 * slot, (turn - 1) & 1, p.err);
         const uint32_t to = tn.ring + slot * bytes, bar = filled + 8 * slot;
-        tc::bar_expect_tx(bar, bytes);
+        tc::bar_expect_tx(bar, bytes - (NR - fetched) * 128);
         const int k = (rank + CLUSTER * j) * BLOCK_K;
         if (whole) tc::tma_load_2d(to + NR * 128, &maps.whole, k, a0, bar);
         for (int t = whole ? total : 0, sec = 0, in = 0; t < total; t += 16) {
@@ -274,7 +277,8 @@ __device__ __forceinline__ void first_product(const AdapterParams& p, const Maps
             tc::tma_load_2d(to + i * 4096, &maps.run, k, rows[32 * i], bar);
           } else {
 #pragma unroll
-            for (int r = 32 * i; r < min(NR, 32 * i + 32); r += 4) tma_gather4(to + r * 128, &maps.x, k, rows[r], rows[r + 1], rows[r + 2], rows[r + 3], bar);
+            for (int r = 32 * i; r < min(NR, 32 * i + 32); r += 4)
+              if (r < fetched) tma_gather4(to + r * 128, &maps.x, k, rows[r], rows[r + 1], rows[r + 2], rows[r + 3], bar);
           }
         }
       }
@@ -704,7 +708,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) adapt
   const int wide = p.sections * p.R;  // numbers of a row of `inner`
   for (int sec0 = 0; sec0 < p.sections; sec0 += together) {
     const int sec1 = min(p.sections, sec0 + together), total = (sec1 - sec0) * R16;
-    first_product(p, maps, (s * p.sections + sec0) * p.R, rows, runs, total, R16, rank, tn, sums);
+    first_product(p, maps, (s * p.sections + sec0) * p.R, rows, runs, count, total, R16, rank, tn, sums);
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     // two neighbouring numbers of a row a thread
     bf16* inner = p.inner + ((long long)tile * SPLITS * LIST + rank * TILE) * wide + sec0 * R16;
@@ -734,11 +738,11 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) adapt
   free_tensor(p, tn);
 }
 
-// ---- many rows, second kernel: 32 rows and a stripe of columns a CTA, 256 columns at a time.  A warp of its own fetches what the pieces need (the
-// rows by TMA, 32 that follow one another a box or four gathered; the columns' rows of B are one stretch), several pieces ahead; eight
-// warps multiply, add and write 32 columns each.  What is on its way is in shared memory, not in registers.  2,048 rows of 6144 columns, rank 16 (50
-// MB) 20 us; 1,057 rows on 24 adapters of rank 64, 28672 columns (238 MB) some 115 us of 161, of which the products are 32 and the writes 18.
-// Pieces of 128 rows and 64 columns, whose warps stand idle where an adapter has one row, took 145 us there (and 18 for the first).
+// ---- many rows, second kernel, where the inner numbers of 128 rows have no room in shared memory (two sections and more of rank 128, or of a float
+// result): 32 rows and a stripe of columns a CTA, 256 columns at a time.  A warp of its own fetches what the pieces need (the rows by TMA, 32
+// that follow one another a box or four gathered; the columns' rows of B are one stretch), several pieces ahead; eight warps multiply, add
+// and write 32 columns each.  What is on its way is in shared memory, not in registers.  Bound by its products and by their operands' way from
+// shared memory: 1,057 rows on 24 adapters of rank 64, 28672 columns (238 MB), some 115 us.
 constexpr int PIECE = 256;  // columns
 constexpr int ROWS = 32;
 constexpr int MAX_STAGES = 4;
@@ -908,6 +912,264 @@ __global__ void __launch_bounds__(THREADS + 32, KEPT > 1 ? 1 : 2) adapter_outer_
   }
 }
 
+// ---- many rows, second kernel on tcgen05: a CTA an SM, each with 128 rows and a stripe of columns, 128 columns at a time.  The tile's inner
+// numbers (every section, every 16-bit part) stay in shared memory for a stripe.  Four warps fetch the pieces (one of them B), several ahead; a
+// warp multiplies (128 x 128 into one half of tensor memory while the other is read); eight warps add and write: a lane adds 64 columns of one
+// row where the rows lie in shared memory, and the warp writes them from there, 128 bytes a row.  What the table of tiles says decides how many
+// pieces a stripe has: the host does not know how many adapters there are.
+// Replayed calls (sort and both products), and with the kernel above in place of this one: 2,048 rows of one adapter, rank 16, 28672 columns (235
+// MB) 62 us, 119; of two, rank 64, 8192 -> 4096 in float 50, 81; 1,057 rows on 24 adapters, rank 64, 28672 columns (238 MB) 123, 171; 700 rows
+// on 24, rank 16, 6144 columns 35, 31 (tiles of 30 rows: too few to fill the pieces).  Bound by latency: of the first piece (the table, the
+// rows' numbers, their TMA; 4 us), and of a piece's way through three kinds of warps where tiles are many and short.  One warp that fetched, some 90
+// cycles for each four rows, took 143 us for the third; products of all columns for both alternating sections 128 for 143.
+constexpr int SPAN = 128;  // columns of a piece
+constexpr int ADDERS = 8;  // warps that add
+constexpr int FETCHERS = LIST / 32;
+
+struct OuterMaps {
+  CUtensorMap run, row, inner, b;  // the rows that are added to (128 bytes: 32 rows, one row); the inner numbers (64: 128 rows); B (64: 128 rows)
+};
+
+// Pieces do not reach from one section into the next.
+__host__ __device__ __forceinline__ int outer_pieces(const AdapterParams& p) {
+  if (p.alternating) return (p.N + SPAN - 1) / SPAN;
+  int pieces = 0;
+  for (int i = 0; i < MAX_SECTIONS; ++i)
+    if (i < p.sections) pieces += (p.width[i] + SPAN - 1) / SPAN;
+  return pieces;
+}
+
+// Pieces of a stripe, of which CTAs take one to four after another (a lane tries each): a stripe begins with the inner numbers, in the time of some
+// four pieces.
+constexpr int SMS = 148;
+__device__ __forceinline__ int pieces_of_stripe(int tiles, int pieces) {
+  const int stripes = max(1, ((int)(threadIdx.x & 3) + 1) * SMS / tiles), each = (pieces + stripes - 1) / stripes;
+  const int time = (tiles * ((pieces + each - 1) / each) + SMS - 1) / SMS * (each + 4);
+  return (int)(__reduce_min_sync(0xffffffffu, (unsigned)min(time, 65535) << 16 | (unsigned)min(each, 65535)) & 65535u);
+}
+
+template <typename O, int SPLITS>
+__global__ void __launch_bounds__(32 * (ADDERS + FETCHERS + 1), 1) adapter_outer_tensor_kernel(const __grid_constant__ AdapterParams p, const __grid_constant__ OuterMaps maps, int tiles, int stages) {
+  extern __shared__ __align__(1024) char pool[];  // the inner numbers [section][part][64 numbers][LIST][128 bytes]; pieces: [128 bytes' columns][LIST][128 bytes], B [64 numbers][SPAN][128 bytes]
+  __shared__ __align__(16) int rows[LIST];
+  __shared__ unsigned run_of[FETCHERS];
+  __shared__ __align__(8) unsigned long long filled[MAX_STAGES], empty[MAX_STAGES], made[2], taken[2], held_bar;
+  __shared__ uint32_t tmem_slot;
+  constexpr int COLUMNS = 128 / (int)sizeof(O), BOXES = SPAN / COLUMNS, BLOCK = LIST * 128;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < MAX_STAGES; ++i) {
+      tc::bar_init(sm32(filled + i), FETCHERS);
+      tc::bar_init(sm32(empty + i), ADDERS);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::bar_init(sm32(made + i), 1);
+      tc::bar_init(sm32(taken + i), ADDERS);
+    }
+    tc::bar_init(sm32(&held_bar), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&maps.run);
+    prefetch_map(&maps.inner);
+    prefetch_map(&maps.b);
+  }
+  // (tensor memory before the wait: the kernel before has its own by then, and only then lets this one begin; the one after waits for this one's)
+  if (warp == ADDERS) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm32(&tmem_slot)), "r"(2u * SPAN) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+  pdl_launch();
+  pdl_wait();
+  int with = 0, used = 0;  // tiles that have an adapter, all tiles: the former come first
+  int3 mine = make_int3(-1, 0, 0);
+  for (int i = 0; i < tiles; i += 32) {
+    const int* t = p.tiles + 3 * (i + lane);
+    const int3 at = i + lane < tiles ? make_int3(t[0], t[1], t[2]) : make_int3(-1, 0, 0);
+    if (i == 0) mine = at;
+    with += __popc(__ballot_sync(0xffffffffu, at.z > 0 && at.x >= 0));
+    used += __popc(__ballot_sync(0xffffffffu, at.z > 0));
+  }
+  if (threadIdx.x < THREADS)
+    for (int t = with; t < used; ++t) copy_rows<O>(p, p.rows + p.tiles[3 * t + 1], p.tiles[3 * t + 2], blockIdx.x, gridDim.x);
+  const int all = outer_pieces(p), stripe = pieces_of_stripe(max(1, with), all), stripes = (all + stripe - 1) / stripe;
+  const int held_blocks = (p.R + 63) / 64;
+  const int part_bytes = held_blocks * BLOCK, ring = p.sections * SPLITS * part_bytes, b_bytes = held_blocks * SPAN * 128, stage_bytes = BOXES * BLOCK + b_bytes;
+  // piece i: its first column, how many it has, its section
+  const auto piece = [&](int i, int& c0, int& end, int& sec) {
+    sec = 0, c0 = i * SPAN, end = min(SPAN, p.N - c0);
+    if (p.alternating) return;
+#pragma unroll
+    for (int k = 0; k < MAX_SECTIONS; ++k) {
+      const int pieces = k < p.sections ? (p.width[k] + SPAN - 1) / SPAN : 0;
+      if (i >= 0 && i < pieces) sec = k, c0 = p.begin[k] + i * SPAN, end = min(SPAN, p.width[k] - i * SPAN);
+      i -= pieces;
+    }
+  };
+  int c0, end, sec;
+  int slot = 0, turn = 0, done = 0, begun = 0;  // the ring, pieces and stripes so far: what phases the barriers are in
+  for (int unit = blockIdx.x; unit < with * stripes; unit += gridDim.x) {
+    const int tile = unit / stripes, left = unit % stripes * stripe, right = min(all, left + stripe);
+    int s = __shfl_sync(0xffffffffu, mine.x, tile & 31), first = __shfl_sync(0xffffffffu, mine.y, tile & 31), count = __shfl_sync(0xffffffffu, mine.z, tile & 31);
+    if (tile >= 32) s = p.tiles[3 * tile], first = p.tiles[3 * tile + 1], count = p.tiles[3 * tile + 2];
+    if (unit != (int)blockIdx.x) __syncthreads();  // (the stripe before is done with the rows and the inner numbers)
+    if (warp < FETCHERS) {
+      const int row = p.rows[first + min((int)threadIdx.x, count - 1)];  // (rows past the last are fetched and not used)
+      const bool run = __all_sync(0xffffffffu, row == __shfl_sync(0xffffffffu, row, 0) + lane);
+      rows[threadIdx.x] = row;
+      if (lane == 0) run_of[warp] = run;
+    }
+    __syncthreads();
+    const int R = p.ranks ? min(max(p.ranks[s], 0), p.R) : p.R;
+    if (R == 0) {
+      if (threadIdx.x < THREADS) copy_rows<O>(p, rows, count, unit % stripes, stripes);
+      continue;
+    }
+    const int R16 = (R + 15) & ~15, blocks = (R16 + 63) / 64;
+    if (warp >= ADDERS && warp < ADDERS + FETCHERS) {
+      // 32 rows a warp, which takes some 90 cycles for each copy that it starts; the first fetches the inner numbers and B too
+      const int part = warp - ADDERS, r0 = 32 * part;
+      const bool run = run_of[part], issues = elect_one();
+      const int fetched = r0 >= count ? 0 : run ? 32 : (min(32, count - r0) + 3) / 4 * 4;
+      if (part == 0 && issues) {
+        const uint32_t held = sm32(&held_bar);
+        tc::bar_expect_tx(held, p.sections * SPLITS * blocks * BLOCK);
+        for (int i = 0; i < p.sections; ++i)
+          for (int t = 0; t < SPLITS; ++t)
+            for (int k = 0; k < blocks; ++k) tc::tma_load_2d(sm32(pool) + (i * SPLITS + t) * part_bytes + k * BLOCK, &maps.inner, i * R16 + 64 * k, (tile * SPLITS + t) * LIST, held);
+      }
+      for (int i = left; i < right; ++i) {
+        piece(i, c0, end, sec);
+        if (issues) {
+          if (turn) tc::bar_wait(sm32(empty + slot), (turn - 1) & 1, p.err);
+          const uint32_t bar = sm32(filled + slot), at = sm32(pool) + ring + slot * stage_bytes;
+          const int boxes = (end + COLUMNS - 1) / COLUMNS;
+          tc::bar_expect_tx(bar, boxes * fetched * 128 + (part == 0 ? blocks * SPAN * 128 : 0));
+          if (part == 0)
+            for (int k = 0; k < blocks; ++k) tc::tma_load_2d(at + BOXES * BLOCK + k * SPAN * 128, &maps.b, 64 * k, s * p.N + c0, bar);
+          for (int k = 0; k < boxes && fetched; ++k) {
+            const uint32_t to = at + k * BLOCK + r0 * 128;
+            if (run) {
+              tc::tma_load_2d(to, &maps.run, c0 + k * COLUMNS, rows[r0], bar);
+            } else {
+              for (int r = 0; r < fetched; r += 4) {
+                const int4 four = *reinterpret_cast<const int4*>(rows + r0 + r);
+                tma_gather4(to + r * 128, &maps.row, c0 + k * COLUMNS, four.x, four.y, four.z, four.w, bar);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (++slot == stages) slot = 0, ++turn;
+      }
+    } else if (warp == ADDERS + FETCHERS) {
+      tc::bar_wait(sm32(&held_bar), begun++ & 1, p.err);
+      for (int i = left; i < right; ++i, ++done) {
+        piece(i, c0, end, sec);
+        tc::bar_wait(sm32(filled + slot), turn & 1, p.err);
+        const int half = done & 1;
+        if (done >= 2) tc::bar_wait(sm32(taken + half), (done / 2 - 1) & 1, p.err);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (elect_one()) {
+          const uint32_t at = sm32(pool) + ring + slot * stage_bytes + BOXES * BLOCK;
+          // where two sections alternate, each takes every second eight rows of B (descriptors of 2,048 bytes from eight to eight)
+          const int alternating = p.alternating ? 1 : 0;
+          for (int h = 0; h <= alternating; ++h) {
+            uint32_t accumulate = 0;
+            for (int t = 0; t < SPLITS; ++t)
+              for (int k = 0; k < R16 / 16; ++k) {
+                const uint64_t da = tc::sdesc(sm32(pool) + ((alternating ? h : sec) * SPLITS + t) * part_bytes + k / 4 * BLOCK) + 2 * (k % 4);
+                const uint64_t db = tc::sdesc(at + k / 4 * SPAN * 128 + h * 1024) + 2 * (k % 4) + ((uint64_t)(alternating * (1024 >> 4)) << 32);
+                tc::umma(tmem + half * SPAN + h * (SPAN / 2), da, db, alternating ? tc::idesc(SPAN / 2, 0) : tc::idesc(SPAN, 0), accumulate);
+                accumulate = 1;
+              }
+          }
+          tc::umma_commit(sm32(made + half));
+        }
+        __syncwarp();
+        if (++slot == stages) slot = 0, ++turn;
+      }
+    } else {
+      // warp w: rows 32 (w % 4) on, columns 64 (w / 4) on
+      const int quarter = warp & 3, columns0 = (warp >> 2) * 64, r = quarter * 32 + lane;
+      for (int i = left; i < right; ++i, ++done) {
+        piece(i, c0, end, sec);
+        const int half = done & 1;
+        tc::bar_wait(sm32(filled + slot), turn & 1, p.err);
+        tc::bar_wait(sm32(made + half), done / 2 & 1, p.err);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        char* at = pool + ring + slot * stage_bytes;
+        if (quarter * 32 < count && columns0 < end) {
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            const int c = columns0 + part * 32;
+            const uint32_t from = tmem + half * SPAN + ((uint32_t)(quarter * 32) << 16);
+            uint32_t v[32];
+            if (p.alternating) {
+              uint32_t w[2][16];
+              tmem_ld16(from + c / 2, w[0]);
+              tmem_ld16(from + SPAN / 2 + c / 2, w[1]);
+              tmem_wait16(w[0]);
+              tmem_wait16(w[1]);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = w[e >> 3 & 1][(e >> 4) * 8 + (e & 7)];
+            } else {
+              tc::tmem_ld32(from + c, v);
+              tc::tmem_wait(v);
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 16 / (int)sizeof(O)) {
+              const int byte = (c + e) * (int)sizeof(O);
+              uint4* old = reinterpret_cast<uint4*>(at + byte / 128 * BLOCK + tc::sw128(r, byte % 128 / 16));
+              uint4 o = *old;
+              if constexpr (sizeof(O) == 2) {
+                float f[8];
+                bf16x8_to_float(o, f);
+                o.x = tc::pk(f[0] + __uint_as_float(v[e]), f[1] + __uint_as_float(v[e + 1]));
+                o.y = tc::pk(f[2] + __uint_as_float(v[e + 2]), f[3] + __uint_as_float(v[e + 3]));
+                o.z = tc::pk(f[4] + __uint_as_float(v[e + 4]), f[5] + __uint_as_float(v[e + 5]));
+                o.w = tc::pk(f[6] + __uint_as_float(v[e + 6]), f[7] + __uint_as_float(v[e + 7]));
+              } else {
+                o.x = __float_as_uint(__uint_as_float(o.x) + __uint_as_float(v[e]));
+                o.y = __float_as_uint(__uint_as_float(o.y) + __uint_as_float(v[e + 1]));
+                o.z = __float_as_uint(__uint_as_float(o.z) + __uint_as_float(v[e + 2]));
+                o.w = __float_as_uint(__uint_as_float(o.w) + __uint_as_float(v[e + 3]));
+              }
+              *old = o;
+            }
+          }
+          __syncwarp();
+          // eight lanes a row of 128 bytes
+          const int chunk = lane & 7;
+#pragma unroll
+          for (int k = 0; k < 64 / COLUMNS; ++k) {
+            const int box = columns0 / COLUMNS + k, c = box * COLUMNS + chunk * 16 / (int)sizeof(O);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int rr = quarter * 32 + i * 4 + (lane >> 3);
+              const uint4 o = *reinterpret_cast<const uint4*>(at + box * BLOCK + tc::sw128(rr, chunk));
+              if (rr < count && c < end) *reinterpret_cast<uint4*>(reinterpret_cast<O*>(p.out) + rows[rr] * p.out_stride + c0 + c) = o;
+            }
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        tc::fence_async_smem();  // what was written here comes before what is copied here next
+        __syncwarp();
+        if (lane == 0) {
+          tc::bar_arrive(sm32(taken + half));
+          tc::bar_arrive(sm32(empty + slot));
+        }
+        if (++slot == stages) slot = 0, ++turn;
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == ADDERS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * SPAN) : "memory");
+}
+
 // Few rows: slots a warp (one where it has one block, or where two keep a second CTA off the SM), the stage, and the bytes for it, the sums and
 // the inner numbers.
 template <typename T, typename O>
@@ -963,35 +1225,53 @@ int make_maps(const AdapterParams& p, Maps& maps) {
              ? 0 : (int)cudaErrorInvalidValue;
 }
 
+// A tensor map of rows of 128 bytes, swizzled.
+template <typename E>
+bool map_rows(CUtensorMap* map, const void* at, long long columns, long long rows, long long stride, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * sizeof(E)};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / sizeof(E)), (cuuint32_t)box_rows}, ones[2] = {1, 1};
+  return tc::encode_tiled()(map, sizeof(E) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(at), dims, strides, box, ones,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename O, int SPLITS>
 int run_wide(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
-  RowMaps base;
-  constexpr int COLUMNS = 128 / (int)sizeof(O);
-  for (int i = 0; i < 2; ++i) {
-    const cuuint64_t dims[2] = {(cuuint64_t)p.N, (cuuint64_t)p.n}, strides[1] = {(cuuint64_t)p.base_stride * sizeof(O)};
-    const cuuint32_t box[2] = {(cuuint32_t)COLUMNS, i ? 1u : 32u}, ones[2] = {1, 1};
-    if (tc::encode_tiled()(i ? &base.row : &base.run, sizeof(O) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(p.base), dims,
-                           strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return (int)cudaErrorInvalidValue;
-  }
-  // (2,048 float rows on eight adapters of rank 32, 4096 columns: 42 us so, 63 with more numbers in registers and one CTA an SM; 2,048 of rank 64: 91
-  // and 81)
-  const bool few_ranks = p.R <= 32;
-  const size_t one = many_smem(p), stage = (size_t)PIECE * sizeof(O) * ROWS + (size_t)PIECE * p.R * 2;
-  const int places = few_ranks ? 2 : 1;  // CTAs an SM: more inner numbers in registers leave room for one
-  const int stages = min(MAX_STAGES, (int)(220 * 1024 / places / stage));  // (of 96 KB at the most: two at least)
+  OuterMaps outer;
+  if (!map_rows<O>(&outer.run, p.base, p.N, p.n, p.base_stride, 32) || !map_rows<O>(&outer.row, p.base, p.N, p.n, p.base_stride, 1)) return (int)cudaErrorInvalidValue;
+  const size_t one = many_smem(p);
   const auto inner = adapter_inner_kernel<SPLITS>;
-  const auto outer = few_ranks ? adapter_outer_kernel<O, SPLITS, 1> : adapter_outer_kernel<O, SPLITS, 4>;
   cudaError_t rc = cudaFuncSetAttribute(inner, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one);
-  if (rc == cudaSuccess) rc = cudaFuncSetAttribute(outer, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages * stage));
   if (rc != cudaSuccess) return (int)rc;
   const int r = launch(inner, dim3(tiles * CLUSTER), dim3(THREADS), one, st, p, maps);
   if (r) return r;
+
+  // on tcgen05, where the inner numbers of a tile and two pieces have room (and rows of B are counted in 31 bits)
+  const size_t parts = (p.R + 63) / 64, held = (size_t)p.sections * SPLITS * parts * LIST * 128, fed = (size_t)SPAN * sizeof(O) * LIST + parts * SPAN * 128;
+  if (held + 2 * fed <= 224 * 1024 && (long long)p.S * p.N <= 0x7fffffff - SPAN) {
+    const long long wide = (long long)p.sections * p.R;
+    if (!map_rows<bf16>(&outer.inner, p.inner, wide, (long long)tiles * SPLITS * LIST, wide, LIST) || !map_rows<bf16>(&outer.b, p.b, p.R, (long long)p.S * p.N, p.R, SPAN))
+      return (int)cudaErrorInvalidValue;
+    const auto kernel = adapter_outer_tensor_kernel<O, SPLITS>;
+    const int stages = min(MAX_STAGES, (int)((224 * 1024 - held) / fed));
+    rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(held + stages * fed));
+    if (rc != cudaSuccess) return (int)rc;
+    return launch(kernel, dim3(SMS), dim3(32 * (ADDERS + FETCHERS + 1)), held + stages * fed, st, p, outer, tiles, stages);
+  }
+
+  // Two CTAs an SM where few inner numbers stay in registers (2,048 float rows on eight adapters, 4096 columns of rank 32: 42 us so, 63 with one CTA and
+  // more numbers; 2,048 of rank 64: 91 and 81).
+  const bool few_ranks = sizeof(O) == 4 && p.R <= 32;
+  const int places = few_ranks ? 2 : 1;
+  const size_t stage = (size_t)PIECE * sizeof(O) * ROWS + (size_t)PIECE * p.R * 2;
+  const int stages = min(MAX_STAGES, (int)(220 * 1024 / places / stage));  // (of 96 KB at the most: two at least)
+  auto kernel = adapter_outer_kernel<O, SPLITS, 4>;
+  if constexpr (sizeof(O) == 4) kernel = few_ranks ? adapter_outer_kernel<O, SPLITS, 1> : kernel;
+  rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages * stage));
+  if (rc != cudaSuccess) return (int)rc;
   // pieces of a CTA: as many as leave a CTA for every place there is
   const int pieces = (p.N + PIECE - 1) / PIECE, full = (p.n + ROWS - 1) / ROWS;
-  const int stripe = max(1, min(pieces, (int)(((long long)pieces * full + places * 148 - 1) / (places * 148))));
-  return launch(outer, dim3((pieces + stripe - 1) / stripe, tiles * (LIST / ROWS)), dim3(THREADS + 32), stages * stage, st, p, base, stripe, stages);
+  const int stripe = max(1, min(pieces, (int)(((long long)pieces * full + places * SMS - 1) / (places * SMS))));
+  return launch(kernel, dim3((pieces + stripe - 1) / stripe, tiles * (LIST / ROWS)), dim3(THREADS + 32), stages * stage, st, p, RowMaps{outer.run, outer.row}, stripe, stages);
 }
 
 // ---- the rows of a step by adapter: one CTA.  Rows without an adapter come last.  The rows of an adapter keep their order within a

@@ -136,6 +136,46 @@ def test_adapter_add_many_rows(ops, dtype, n, kind):
         assert torch.equal(run(ops, x, bank, ids, base), base)
 
 
+@pytest.mark.parametrize(
+    "k,ends,rank,wide",
+    [
+        (64, (8, 16, 24), 16, False), (200, (136, 272, 408), 48, False), (264, (1000,), 128, False), (136, (520, 1032), 128, False), (136, (72, 80, 664), 112, False),
+        (136, (520,), 64, True), (136, (136, 408), 32, True), (72, (264, 400), 64, True), (136, (3008,), 128, True),
+    ],
+)  # fmt: skip
+def test_adapter_add_many_rows_of_every_shape(ops, k, ends, rank, wide):
+    """Sections that end inside a piece, inner numbers that have room and that have none, ranks below the bank's, both results."""
+    n = 901
+    bank = make(ops, 4, k, ends, rank, torch.bfloat16, ranks=[rank, rank - 5, 0, 3])
+    x, base = inputs(n, k, ends[-1], torch.bfloat16, wide)
+    for ids in (mixed_ids(n, 4), [i * 4 // n for i in range(n)], [1] * 897 + [-1] * 4):
+        want, mag = formula(x, bank, ids, base)
+        for in_place in (False, True):
+            close(run(ops, x, bank, ids, base, in_place), want, mag, base.dtype)
+
+
+@pytest.mark.parametrize("half,n", [(8, 700), (136, 700), (1000, 2100)])
+def test_adapter_add_many_rows_alternating(ops, half, n):
+    bank = make(ops, 40, 136, (half, 2 * half), 24, torch.bfloat16, alternating=True)
+    x, base = inputs(n, 136, 2 * half, torch.bfloat16, False)
+    for ids in (mixed_ids(n, 40), [i % 40 for i in range(n)]):
+        want, mag = formula(x, bank, ids, base)
+        close(run(ops, x, bank, ids, base), want, mag, base.dtype)
+
+
+def test_adapter_add_of_one_row_of_any_stride(ops):
+    """How far it is to a row that there is not does not matter."""
+    bank = make(ops, 2, 64, (64,), 16, torch.bfloat16)
+    x, base = inputs(1, 64, 64, torch.bfloat16, False)
+    want, mag = formula(x, bank, [1], base)
+    one = lambda t: t.as_strided((1, 64), (3, 1))  # noqa: E731
+    groups = ops.AdapterGroups(1, 2, "cuda")
+    ops.group_by_adapter(torch.ones(1, dtype=torch.int32, device="cuda"), groups)
+    out = torch.full_like(base, float("nan"))
+    ops.adapter_add(one(x), bank, groups, one(out), base=one(base))
+    close(out, want, mag, base.dtype)
+
+
 def test_adapter_rows_without_an_adapter_stay_as_they_are(ops):
     bank = make(ops, 2, 64, (64,), 16, torch.bfloat16)
     for n in (3, 40, 600):

@@ -51,6 +51,9 @@ def test_adapter_call_refusals():
     ):  # fmt: skip
         with pytest.raises(ValueError):
             ops.adapter_add(x_, bank, groups, out_, base=base_)
+    for x_, out_, base_ in ((x[:1].expand(4, 64), out, None), (x, out[:1].expand(4, 64), None), (x, out, out[:1].expand(4, 64))):  # rows that are one
+        with pytest.raises(ValueError):
+            ops.adapter_add(x_, bank, groups, out_, base=base_)
     with pytest.raises(ValueError, match="groups"):
         ops.adapter_add(x, ops.AdapterBank(*bank_args(s=3, sections=1)), groups, out)
     with pytest.raises(RuntimeError, match="CUDA"):
