@@ -2891,9 +2891,10 @@ class AdapterBank:
 
 
 ADAPTER_DIRECT = 64  # up to so many rows the kernels group for themselves
-# from so many bfloat16 rows on the two products are kernels of their own (4096 x 4096, rank 16: 512 rows 13 us in one kernel and 18 in two,
-# 2,048 rows 44 and 34; 4096 x 28672: 700 rows 56 and 42)
-ADAPTER_MANY = 640
+# from so many bfloat16 rows on the two products are kernels of their own: 32 clusters of 16 rows find room at the same time (one adapter of rank
+# 16, 4096 x 6144: 512 rows 16 us in one kernel and 22 in two, 600 rows 24 and 24; 4096 x 28672: 29 and 30, 49 and 34; 20 of rank 64 there: 116 and
+# 88, 119 and 98)
+ADAPTER_MANY = 513
 ADAPTER_TILE = 128  # rows of one adapter that a tile of the list has room for
 
 

@@ -154,7 +154,7 @@ def test_adapter_add_many_rows_of_every_shape(ops, k, ends, rank, wide):
             close(run(ops, x, bank, ids, base, in_place), want, mag, base.dtype)
 
 
-@pytest.mark.parametrize("half,n", [(8, 700), (136, 700), (1000, 2100)])
+@pytest.mark.parametrize("half,n", [(8, 700), (136, 512), (136, 513), (136, 700), (1000, 2100)])
 def test_adapter_add_many_rows_alternating(ops, half, n):
     bank = make(ops, 40, 136, (half, 2 * half), 24, torch.bfloat16, alternating=True)
     x, base = inputs(n, 136, 2 * half, torch.bfloat16, False)
