@@ -205,8 +205,12 @@ class BeamSearch:
             items, ends = [], []
             for group, seq, adapter in waiting:
                 start = done[seq]
-                take = min(len(group.prompt) - start, budget, self.cfg.max_prefill_chunk or budget)
-                if take < 1 or len(items) >= rt.max_seqs or (not self.cfg.enable_chunked_prefill and take < len(group.prompt)):
+                take = min(len(group.prompt) - start, budget)
+                if self.cfg.enable_chunked_prefill:
+                    take = min(take, self.cfg.max_prefill_chunk or take)
+                elif take < len(group.prompt):
+                    break
+                if take < 1 or len(items) >= rt.max_seqs:
                     break
                 self.bm.append_slots(seq, start + take, start)
                 last = start + take == len(group.prompt)

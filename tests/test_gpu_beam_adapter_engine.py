@@ -311,6 +311,20 @@ def test_beams_of_models_with_states_and_windows(tmp_path, preset, dtype):
     engine.block_manager.check_invariants()
 
 
+def test_beam_search_of_prompts_cut_and_whole(folders):
+    """How prompts come to their steps changes nothing, the cap on a portion without portions included."""
+    from kvforge_b200 import BeamParams
+
+    name = "tiny-a"
+    prompts = prompts_for(name, [20, 18, 25, 3, 40], seed=5)
+    outs = []
+    for sched in (dict(), dict(max_prefill_chunk=8), dict(max_num_batched_tokens=48, enable_chunked_prefill=False, max_prefill_chunk=8)):
+        engine = engine_for(folders[name], name, **sched)
+        found = engine.beam_search(prompts, BeamParams(num_beams=2, max_tokens=4, num_return=2, ignore_eos=True))
+        outs.append([[h.token_ids for h in o.hypotheses] for o in found])
+    assert outs[0] == outs[1] == outs[2]
+
+
 def test_beam_search_refusals_and_pressure(folders):
     from kvforge_b200 import BeamParams
     from kvforge_b200.engine.scheduler import RequestRejectedError
