@@ -45,8 +45,8 @@ class BeamParams:
             raise ValueError("max_tokens must be >= 1")
         if not 1 <= self.num_return <= self.num_beams:
             raise ValueError("num_return must be between 1 and num_beams")
-        if not math.isfinite(self.length_penalty):
-            raise ValueError("length_penalty must be finite")
+        if not abs(self.length_penalty) <= 64:  # (a length to that power is still a float)
+            raise ValueError("length_penalty must lie between -64 and 64")
 
 
 @dataclass

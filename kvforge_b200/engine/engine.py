@@ -212,6 +212,8 @@ class InferenceEngine:
             if len(per_prompt) != len(prompts):
                 raise ValueError(f"{len(per_prompt)} sampling parameter sets for {len(prompts)} prompts")
         chosen = self._per_prompt(adapters, len(prompts))
+        for a in chosen:
+            self._adapter_slot(a)  # (a name that means none leaves no request behind)
         names = [self.add_request(prompt, sp, adapter=a) for prompt, sp, a in zip(prompts, per_prompt, chosen)]
         final: dict[str, RequestOutput] = {}
         while self.has_unfinished_requests():

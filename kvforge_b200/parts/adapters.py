@@ -11,6 +11,7 @@ alone.
 from __future__ import annotations
 
 import json
+import math
 from pathlib import Path
 
 import torch
@@ -113,6 +114,8 @@ class AdapterStore:
         places = {proj: (d, i) for d in self._declared for i, proj in enumerate(d.names)}
         if not pairs:
             raise AdapterError("the adapter has no tensors")
+        if not math.isfinite(scale):
+            raise AdapterError(f"the adapter's scale is {scale}")
         for proj, ab in pairs.items():
             if proj not in places:
                 raise AdapterError(f"{proj} takes no adapters in this model")
@@ -120,7 +123,7 @@ class AdapterStore:
                 raise AdapterError(f"{proj} needs both lora_A and lora_B")
             d, i = places[proj]
             a, b = ab["A"], ab["B"]
-            r = a.shape[0]
+            r = a.shape[0] if a.dim() else 0
             if a.dim() != 2 or b.dim() != 2 or tuple(a.shape) != (r, d.bank.k) or tuple(b.shape) != (d.widths[i], r) or r < 1:
                 raise AdapterError(f"{proj}: lora_A {tuple(a.shape)} and lora_B {tuple(b.shape)} do not fit [{d.widths[i]}, {d.bank.k}]")
             if r > self.max_rank:

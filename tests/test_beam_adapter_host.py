@@ -14,7 +14,7 @@ from kvforge_b200.cache.state_slots import StateSlotPool
 from kvforge_b200.engine.beam import BeamGroup, _Beam
 from kvforge_b200.engine.request import FinishReason
 from kvforge_b200.engine.step import BatchItem, _Layout
-from kvforge_b200.parts.adapters import AdapterError, read_adapter
+from kvforge_b200.parts.adapters import AdapterError, AdapterStore, read_adapter
 from kvforge_b200.weights.safetensors_io import write_safetensors
 
 
@@ -167,7 +167,7 @@ def test_length_penalty():
 
 
 def test_beam_parameter_refusals():
-    for kw in (dict(num_beams=0), dict(num_beams=33), dict(max_tokens=0), dict(num_return=0), dict(num_beams=2, num_return=3), dict(length_penalty=float("inf"))):
+    for kw in (dict(num_beams=0), dict(num_beams=33), dict(max_tokens=0), dict(num_return=0), dict(num_beams=2, num_return=3), dict(length_penalty=float("inf")), dict(length_penalty=float("nan")), dict(length_penalty=1e4)):
         with pytest.raises(ValueError):
             BeamParams(**kw)
 
@@ -195,6 +195,32 @@ def test_read_adapter(tmp_path):
             read_adapter(tmp_path)
     (tmp_path / "adapter_config.json").write_text(json.dumps({"r": 4, "lora_alpha": 8, "use_rslora": True}))
     assert read_adapter(tmp_path)[1] == 4.0
+
+
+def test_adapter_store_refusals():
+    store = AdapterStore(2, 8, 16, torch.float32, torch.device("cpu"))
+    store.declare(["q", "k"], [16, 8], 8)
+    a, b = torch.randn(4, 8), torch.randn(16, 4)
+    good = {"q.lora_A.weight": a, "q.lora_B.weight": b}
+    for bad in (
+        {}, {"q.lora_A.weight": a}, {**good, "q.bias": b}, {"v.lora_A.weight": a, "v.lora_B.weight": b}, {**good, "q.lora_A.weight": torch.tensor(1.0)},
+        {**good, "q.lora_B.weight": torch.randn(4)}, {**good, "q.lora_B.weight": torch.randn(8, 4)}, {"q.lora_A.weight": torch.randn(9, 8), "q.lora_B.weight": torch.randn(16, 9)},
+    ):  # fmt: skip
+        with pytest.raises(AdapterError):
+            store.load("x", bad, 1.0)
+    with pytest.raises(AdapterError):
+        store.load("x", good, float("nan"))
+    assert not store.slots
+    assert store.load("x", good, 2.0) == 0 and store.load("y", good, 1.0) == 1
+    for name in ("x", "z"):
+        with pytest.raises(AdapterError):
+            store.load(name, good, 1.0)
+    store.unload("x")
+    with pytest.raises(AdapterError):
+        store.unload("x")
+    with pytest.raises(AdapterError):
+        store.slot("x")
+    assert store.load("z", good, 1.0) == 0 and store.slot("z") == 0 and store.slot(None) == -1
 
 
 def test_a_steps_layout_carries_adapters_only_where_some_are_kept():

@@ -311,6 +311,13 @@ def test_beams_of_models_with_states_and_windows(tmp_path, preset, dtype):
     engine.block_manager.check_invariants()
 
 
+def test_generate_with_an_unknown_adapter_leaves_nothing_behind(folders):
+    engine = engine_for(folders["tiny-a"], "tiny-a")
+    with pytest.raises(ValueError):
+        engine.generate([[1, 2], [3]], greedy(2), adapters=[None, "none of them"])
+    assert not engine.has_unfinished_requests()
+
+
 def test_beam_search_of_prompts_cut_and_whole(folders):
     """How prompts come to their steps changes nothing, the cap on a portion without portions included."""
     from kvforge_b200 import BeamParams
