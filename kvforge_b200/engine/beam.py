@@ -45,7 +45,7 @@ class BeamParams:
             raise ValueError("max_tokens must be >= 1")
         if not 1 <= self.num_return <= self.num_beams:
             raise ValueError("num_return must be between 1 and num_beams")
-        if not abs(self.length_penalty) <= 64:  # (a length to that power is still a float)
+        if not abs(self.length_penalty) <= 64:
             raise ValueError("length_penalty must lie between -64 and 64")
 
 
@@ -77,6 +77,9 @@ class BeamGroup:
     def __init__(self, prompt: list[int], params: BeamParams, stops: set[int], limit: int) -> None:
         self.prompt, self.params, self.stops = prompt, params, stops
         self.limit = limit  # tokens a hypothesis may have
+        # scores are doubles above their smallest normal number, 2^-1022: sums of log probabilities lie between 2^-149 and 104 a token
+        if abs(params.length_penalty) * math.log2(limit) > 870:
+            raise RequestRejectedError(f"length_penalty = {params.length_penalty} has no scores for hypotheses of up to {limit} tokens")
         self.beams: list[_Beam] = []
         self.finished: list[BeamHypothesis] = []
         self.done = False
