@@ -1192,6 +1192,12 @@ size_t few_smem(AdapterParams& p, int splits) {
   return rest + p.stage;
 }
 
+// Tensor memory has 512 columns, four CTAs' of the inner kernel.  A fifth on the same SM would wait for some with the CTAs of its cluster
+// waiting for it, theirs kept: clusters that have them on different SMs could wait for one another for good.  So each CTA takes at least so much shared
+// memory that a fifth has no room.  (Up to 512 columns of k one block is all that a CTA has, and six CTAs of rank 16 found room.)
+constexpr int INNER_LEAST = 46 * 1024;
+static_assert(512 / LIST == 4 && 5 * (INNER_LEAST + 1024) > 228 * 1024, "a fifth CTA has no room (each has 1 KB besides what it asks for)");
+
 // Many rows: blocks of k that shared memory holds, columns of tensor memory, and the bytes for the ring and the sums (16 KB at least: the last
 // lanes of the accumulator read past the rows of A).
 size_t many_smem(AdapterParams& p) {
@@ -1202,7 +1208,7 @@ size_t many_smem(AdapterParams& p) {
   const int two = rest < 112 * 1024 ? (int)((112 * 1024 - rest) / slot) : 0, one = (int)((220 * 1024 - rest) / slot);
   p.slots = max(1, min(min(two >= 3 ? two : one, MAX_SLOTS), blocks));
   p.tmem = LIST;
-  return p.slots * slot + rest;
+  return max(p.slots * slot + rest, (size_t)INNER_LEAST);
 }
 static_assert(MOST <= 128 && CLUSTER * MOST * SUM_ROW * 4 + 16 * 1024 + slot_bytes(LIST, MOST) <= 220 * 1024, "one tile of the accumulator; room for a block");
 static_assert(CLUSTER * TILE * MOST * 4 + 3 * TILE * (MOST + 16) * 2 + WARPS * slot_bytes(TILE, MOST) <= 226 * 1024, "room for a block a warp");
@@ -1375,6 +1381,13 @@ int run_tiles(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
 KVF_API int kvf_adapters_set_pdl(int on) {
   g_pdl_enabled = on;
   return 0;
+}
+
+// Bytes of shared memory of a CTA that makes the inner numbers of many rows.
+KVF_API int kvf_adapter_inner_bytes(int sections, int R, int K) {
+  AdapterParams p{};
+  p.sections = sections, p.R = R, p.K = K, p.most = min(sections, MOST / R) * R;
+  return (int)many_smem(p);
 }
 
 KVF_API int kvf_adapter_group(const int* ids, int n, int S, int tile, int max_tiles, int* rows, int* tiles, int* err, cudaStream_t st) {

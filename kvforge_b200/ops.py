@@ -102,6 +102,7 @@ _SIGNATURES = {
     "kvf_adapter_add_{s}": "plppiplplippipipp",
     "kvf_adapter_group": "piiiipppp",
     "kvf_adapters_set_pdl": "i",
+    "kvf_adapter_inner_bytes": "iii",
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 
