@@ -595,7 +595,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS, 2) ad
 #pragma unroll
         for (int c = 0; c < CLUSTER; ++c) st_cluster(to, c, v);
       }
-      if (TENSOR) tc::fence_async_smem();  // (before the next sections' copies into the same place)
+      tc::fence_async_smem();  // what was written and read here comes before the copies into the same place: the columns', the next sections'
       __syncthreads();
     }
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
