@@ -133,7 +133,8 @@ class BeamSearch:
         self.adapters = adapter_slot
         self._count = itertools.count()
         self._issued: list[str] = []  # names of the requests that hold beams
-        groups = max(1, self.cfg.max_num_seqs // params.num_beams)
+        # a step takes so many beams: one request and one token each
+        groups = max(1, min(self.cfg.max_num_seqs, self.cfg.max_num_batched_tokens) // params.num_beams)
         rows, k = groups * params.num_beams, self.candidates
         dev = self.core.device
         self.max_groups = groups
@@ -272,6 +273,8 @@ class BeamSearch:
                 raise RequestRejectedError(f"a prompt of {len(prompt)} tokens exceeds max_num_batched_tokens = {cfg.max_num_batched_tokens} and prompts are not cut")
             if p.num_beams > cfg.max_num_seqs:
                 raise RequestRejectedError(f"{p.num_beams} beams are more than max_num_seqs = {cfg.max_num_seqs}")
+            if p.num_beams > cfg.max_num_batched_tokens:
+                raise RequestRejectedError(f"{p.num_beams} beams are more than max_num_batched_tokens = {cfg.max_num_batched_tokens}")
             group = BeamGroup(list(prompt), p, self.stops, min(p.max_tokens, cfg.max_model_len - len(prompt)))
             if self._reserve(group.prompt, group.limit) > bm.num_blocks:
                 raise RequestRejectedError(f"{p.num_beams} beams of {len(prompt) + group.limit} tokens can never fit the pages of the cache")
