@@ -140,8 +140,10 @@ class ModelRunner:
         self.n_groups = block_manager.num_groups
         self.cuda_graphs = bool(cuda_graphs)
         self.pdl = bool(pdl)  # programmatic dependent launch between the kernels of a step
-        # the most sequences a step can hold is a bucket of its own, so that no batch size goes without a graph
-        self.graph_buckets = sorted({b for b in graph_buckets if b <= rt.max_seqs} | ({rt.max_seqs} if rt.max_seqs <= max(graph_buckets) else set())) or [rt.max_seqs]
+        # the most sequences a step can hold (each brings a token) is a bucket of its own, so that no batch size goes without a graph;
+        # a bucket beyond it would be padded to more rows than the buffers of a step were made for
+        most = min(rt.max_seqs, rt.max_tokens)
+        self.graph_buckets = sorted({b for b in graph_buckets if b <= most} | ({most} if most <= max(graph_buckets) else set())) or [most]
         # keyed by (tokens, sequences, longest context the graph reaches, single-token sequences in a step of
         # many tokens, decode form, adapters); the form is part of the key because a step of many tokens padded to as many
         # tokens as sequences (64 tokens in 64 sequences) is another graph than 64 decoding sequences

@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from helpers import TINY, make_model_dir
-from test_gpu_beam_adapter_engine import engine_for, prompts_for
+from plain_llama import PlainLlama
+from test_gpu_beam_adapter_engine import engine_for, greedy, make_adapter, merged, prompts_for
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +34,18 @@ def test_beams_of_several_prompts_within_the_tokens_of_a_step(folders, graphs):
     with pytest.raises(RequestRejectedError, match="max_num_batched_tokens"):
         narrow.beam_search(prompts, BeamParams(num_beams=8, max_tokens=6, ignore_eos=True))
     assert narrow.block_manager.num_free_blocks == narrow.block_manager.num_blocks
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_more_requests_than_a_step_has_tokens_for(folders, graphs):
+    """18 decoding requests of 32 places and 20 tokens a step: a captured step has room for more rows than the budget of tokens."""
+    name = "tiny-a"
+    adapter = make_adapter(folders[name], 8, 21)
+    engine = engine_for(folders[name], name, max_num_seqs=32, max_num_batched_tokens=20, cuda_graphs=graphs)
+    engine.load_adapter("it", *adapter)
+    prompts = prompts_for(name, [3 + i % 5 for i in range(18)], seed=90)
+    chosen = ["it" if i % 2 else None for i in range(18)]
+    outs = engine.generate(prompts, greedy(12), adapters=chosen)
+    plains = {None: PlainLlama(folders[name]), "it": merged(folders[name], adapter)}
+    for p, c, o in zip(prompts, chosen, outs):
+        assert o.output_token_ids == plains[c].greedy(p, 12)
