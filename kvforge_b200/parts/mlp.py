@@ -59,6 +59,8 @@ class GatedMLP(FeedForward):
             gu = rt.buf("mlp.gate_up", n, 2 * self.inter)
             if ops.skinny_ok(x, self.w_gate_up):
                 ops.gemm_skinny(x, self.w_gate_up, gu)
+            elif self.interleaved and ops.tcgen05_ok(x, self.w_gate_up):
+                ops.gemm_tcgen05(x, self.w_gate_up, gu, err=rt.err)
             else:
                 ops.linear(x, self.w_gate_up, gu)
             adapters.add(ctx, self.gate_up_bank, x, gu)
