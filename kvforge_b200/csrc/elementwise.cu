@@ -496,14 +496,16 @@ __global__ void silu_mul_kernel(const T* __restrict__ gu, T* __restrict__ out, i
 
 // The same, 8 bfloat16 outputs (one 16-byte load of gates, one of ups, one 16-byte store) per
 // thread; needs I % 8 == 0, which the interleaved layout (blocks of 8) has by construction.
+// With `ids` only for the rows whose id is from 0 to num_ids - 1.
 __global__ void silu_mul_bf16x8_kernel(const bf16* __restrict__ gu, bf16* __restrict__ out, int I, int block,
-                                       size_t groups) {
+                                       size_t groups, const int* __restrict__ ids, int num_ids) {
   pdl_launch();
   pdl_wait();
   const size_t gidx = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (gidx >= groups) return;
   const int per_row = I >> 3;
   const size_t n = gidx / per_row;
+  if (ids && (unsigned)ids[n] >= (unsigned)num_ids) return;
   const int i0 = (int)(gidx - n * per_row) << 3;
   const int cg = block ? (i0 / block) * 2 * block + (i0 % block) : i0;
   const int cu = block ? cg + block : I + i0;
@@ -525,6 +527,29 @@ __global__ void silu_mul_bf16x8_kernel(const bf16* __restrict__ gu, bf16* __rest
   *reinterpret_cast<uint4*>(out + n * (size_t)I + i0) = o;
 }
 
+// The same from gates and ups in float, eight outputs (two 16-byte loads of gates, two of ups) per thread.
+__global__ void silu_mul_float_bf16x8_kernel(const float* __restrict__ gu, bf16* __restrict__ out, int I, int block, size_t groups) {
+  pdl_launch();
+  pdl_wait();
+  const size_t gidx = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (gidx >= groups) return;
+  const int per_row = I >> 3;
+  const size_t n = gidx / per_row;
+  const int i0 = (int)(gidx - n * per_row) << 3;
+  const int cg = block ? (i0 / block) * 2 * block + (i0 % block) : i0;
+  const float4* gp = reinterpret_cast<const float4*>(gu + n * 2 * (size_t)I + cg);
+  const float4* up = reinterpret_cast<const float4*>(gu + n * 2 * (size_t)I + (block ? cg + block : I + i0));
+  const float4 gv[2] = {gp[0], gp[1]}, uv[2] = {up[0], up[1]};
+  uint4 o;
+  __nv_bfloat162* op = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    op[2 * e] = __floats2bfloat162_rn(gv[e].x / (1.f + expf(-gv[e].x)) * uv[e].x, gv[e].y / (1.f + expf(-gv[e].y)) * uv[e].y);
+    op[2 * e + 1] = __floats2bfloat162_rn(gv[e].z / (1.f + expf(-gv[e].z)) * uv[e].z, gv[e].w / (1.f + expf(-gv[e].w)) * uv[e].w);
+  }
+  *reinterpret_cast<uint4*>(out + n * (size_t)I + i0) = o;
+}
+
 template <typename T>
 int launch_silu_mul(const void* gu, void* out, long long N, int I, int block, cudaStream_t st) {
   const size_t total = (size_t)N * I;
@@ -537,7 +562,7 @@ int launch_silu_mul<bf16>(const void* gu, void* out, long long N, int I, int blo
   if ((I & 7) == 0 && (block == 0 || block == 8) && aligned) {
     const size_t groups = total >> 3;
     return launch(silu_mul_bf16x8_kernel, dim3((unsigned)((groups + 255) / 256)), dim3(256), 0, st, (const bf16*)gu,
-                  (bf16*)out, I, block, groups);
+                  (bf16*)out, I, block, groups, (const int*)nullptr, 0);
   }
   return launch(silu_mul_kernel<bf16>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, (const bf16*)gu,
                 (bf16*)out, I, block, total);
@@ -653,6 +678,22 @@ static inline int norm_threads(int H) {
 KVF_API int kvf_set_pdl(int enabled) {
   kvf::g_pdl_enabled = enabled ? 1 : 0;
   return 0;
+}
+
+// bfloat16, for the rows that took an adapter (their id is from 0 to num_ids - 1); the other rows of `out` stay
+KVF_API int kvf_silu_mul_of_rows(const void* gu, void* out, long long N, int I, int block, const int* ids, int num_ids, cudaStream_t st) {
+  const size_t groups = (size_t)N * I >> 3;
+  if (groups == 0) return 0;
+  if ((I & 7) || (block != 0 && block != 8) || !ids || ((((uintptr_t)gu) | ((uintptr_t)out)) & 15)) return (int)cudaErrorInvalidValue;
+  return launch(silu_mul_bf16x8_kernel, dim3((unsigned)((groups + 255) / 256)), dim3(256), 0, st, (const bf16*)gu, (bf16*)out, I, block, groups, ids, num_ids);
+}
+
+// float gates and ups to bfloat16: rows of whole groups of 8, alternating in blocks of 8 or apart
+KVF_API int kvf_silu_mul_float_bf16(const float* gu, void* out, long long N, int I, int block, cudaStream_t st) {
+  const size_t groups = (size_t)N * I >> 3;
+  if (groups == 0) return 0;
+  if ((I & 7) || (block != 0 && block != 8) || ((((uintptr_t)gu) | ((uintptr_t)out)) & 15)) return (int)cudaErrorInvalidValue;
+  return launch(silu_mul_float_bf16x8_kernel, dim3((unsigned)((groups + 255) / 256)), dim3(256), 0, st, gu, (bf16*)out, I, block, groups);
 }
 
 KVF_ELEMENTWISE_API(f32, float)

@@ -57,6 +57,10 @@ struct TcParams {
   const int* meta;
   const int* scatter;
   int max_row_tiles;
+  // mode 3 with adapters: rows whose id is from 0 to num_ids - 1 go as they are to rows_out, bfloat16 with ld_rows columns from one to the next
+  const int* ids = nullptr;
+  int num_ids = 0, ld_rows = 0;
+  void* rows_out = nullptr;
 };
 
 __device__ __forceinline__ uint32_t sm_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -276,6 +280,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       const bool row_ok = q * 32 + lane < rows;
       int row = m0 + q * 32 + lane;
       if (p.scatter && row_ok) row = p.scatter[row];
+      const bool apart = p.ids && row_ok && (unsigned)p.ids[row] < (unsigned)p.num_ids;
       if (!mbar_wait(acc_full0 + 8 * b, (j >> 1) & 1, p.err)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -341,7 +346,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
               r[16 * h + i] = __float_as_uint(__fdividef(g, 1.f + __expf(-al * g)) * (u + sh));
             }
         }
-        if (p.mode == 3 || p.mode == 7) {
+        if ((p.mode == 3 || p.mode == 7) && !apart) {
           // columns are weight rows [g0..7, u0..7, g8..15, u8..15]: 16 outputs from 32 columns
           bf16* dst = reinterpret_cast<bf16*>(p.out) + (size_t)row * p.ldo + (col >> 1);
           uint32_t o[8];
@@ -363,7 +368,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
               if (col + 16 * (i >> 3) < p.N) dst[i] = ob[i];  // N is a multiple of 16: whole blocks of [8 g | 8 u]
           }
         } else {
-          bf16* dst = reinterpret_cast<bf16*>(p.out) + (size_t)row * p.ldo + col;
+          bf16* dst = reinterpret_cast<bf16*>(apart ? p.rows_out : p.out) + (size_t)row * (apart ? p.ld_rows : p.ldo) + col;
           if (col + 32 <= p.N) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
@@ -443,13 +448,10 @@ int launch_tc(const CUtensorMap& mx, const CUtensorMap& mw, const TcParams& p, c
 
 }  // namespace
 
-// x: [M, K] (row stride ldx), w: [N, K] (row stride ldw), bfloat16, 16-byte aligned, K % 8 == 0,
-// strides multiples of 8.  mode 0: out bfloat16 [M, N]; mode 3: out bfloat16 [M, N/2] =
-// silu(gate) * up for w in the interleaved gate/up layout (N % 16 == 0); mode 8: out bfloat16 [M, N] =
-// gelu_tanh(y + bias) (bias float [N], 16-byte aligned, or null).  err: device flag
-// (bit 4 is raised if a wait inside the kernel ran out).
-KVF_API int kvf_gemm_tcgen05_bf16(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw,
-                                  int ldo, int mode, const float* bias, int* err, cudaStream_t st) {
+namespace {
+
+int run_gemm(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, int ldo, int mode, const float* bias, const int* ids, int num_ids, void* rows,
+             int ld_rows, int* err, cudaStream_t st) {
   if (M <= 0 || N <= 0) return 0;
   if (K <= 0 || (K & 7) || (ldx & 7) || (ldw & 7) || (ldo & 7) || (mode != 0 && mode != 3 && mode != 8))
     return (int)cudaErrorInvalidValue;
@@ -460,6 +462,7 @@ KVF_API int kvf_gemm_tcgen05_bf16(const void* x, const void* w, void* out, int M
   p.act_limit = p.act_alpha = p.act_shift = 0.f;
   p.bias = bias;
   p.tiles = nullptr; p.meta = nullptr; p.scatter = nullptr; p.max_row_tiles = 0;
+  p.ids = ids; p.num_ids = num_ids; p.rows_out = rows; p.ld_rows = ld_rows;
   CUtensorMap mx, mw;
   int rc = make_map(&mx, x, M, K, ldx, BM);
   if (rc) return rc;
@@ -471,6 +474,26 @@ KVF_API int kvf_gemm_tcgen05_bf16(const void* x, const void* w, void* out, int M
   rc = make_map(&mw, w, N, K, ldw, 128);
   if (rc) return rc;
   return launch_tc<128, 4>(mx, mw, p, st);
+}
+
+}  // namespace
+
+// x: [M, K] (row stride ldx), w: [N, K] (row stride ldw), bfloat16, 16-byte aligned, K % 8 == 0,
+// strides multiples of 8.  mode 0: out bfloat16 [M, N]; mode 3: out bfloat16 [M, N/2] =
+// silu(gate) * up for w in the interleaved gate/up layout (N % 16 == 0); mode 8: out bfloat16 [M, N] =
+// gelu_tanh(y + bias) (bias float [N], 16-byte aligned, or null).  err: device flag
+// (bit 4 is raised if a wait inside the kernel ran out).
+KVF_API int kvf_gemm_tcgen05_bf16(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw,
+                                  int ldo, int mode, const float* bias, int* err, cudaStream_t st) {
+  return run_gemm(x, w, out, M, N, K, ldx, ldw, ldo, mode, bias, nullptr, 0, nullptr, 0, err, st);
+}
+
+// Mode 3 for the rows that take no adapter (their id is not from 0 to num_ids - 1); the others go as they are, bfloat16, to the same rows of
+// `rows` [M, N] (row stride ld_rows), before something is added to them.
+KVF_API int kvf_gemm_silu_apart_bf16(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, int ldo, const int* ids, int num_ids, void* rows,
+                                     int ld_rows, int* err, cudaStream_t st) {
+  if (!ids || !rows || (ld_rows & 7) || (((uintptr_t)rows) & 15)) return (int)cudaErrorInvalidValue;
+  return run_gemm(x, w, out, M, N, K, ldx, ldw, ldo, 3, nullptr, ids, num_ids, rows, ld_rows, err, st);
 }
 
 // The grouped form: x [P, K] with its rows ordered by expert, w [E * N, K], `tiles` / `meta` as a sort on the device

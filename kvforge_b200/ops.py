@@ -23,6 +23,8 @@ _SIGNATURES = {
     "kvf_add_residual_{s}": "pplp",
     "kvf_rope_cache_{s}": "ppilppppppiiiiiilpp",
     "kvf_silu_mul_{s}": "ppliip",
+    "kvf_silu_mul_float_bf16": "ppliip",
+    "kvf_silu_mul_of_rows": "ppliipip",
     "kvf_cast_from_float_{s}": "pplp",
     "kvf_paged_attention_generic_{s}": "pppppppiiiiiiiiiifiiiippiipifpp",
     "kvf_paged_attention_mma_bf16": "pppppppiiiiiiiiifiiiippp",
@@ -37,6 +39,7 @@ _SIGNATURES = {
     "kvf_gemm_skinny_bf16": "pppiiiiiiiilpp",
     "kvf_set_pdl": "i",
     "kvf_gemm_tcgen05_bf16": "pppiiiiiiippp",
+    "kvf_gemm_silu_apart_bf16": "pppiiiiiipipipp",
     "kvf_sample_f32": "pliippppppp",
     "kvf_argmax_f32": "pliipipp",
     "kvf_scale_softcap_f32": "plffp",
@@ -400,19 +403,34 @@ def interleave_gate_up(w_gate: torch.Tensor, w_up: torch.Tensor) -> torch.Tensor
     return torch.stack([w_gate.view(i // b, b, h), w_up.view(i // b, b, h)], dim=1).reshape(2 * i, h).contiguous()
 
 
-def silu_mul(gate_up: torch.Tensor, out: torch.Tensor, interleaved: bool = False) -> None:
+def silu_mul(gate_up: torch.Tensor, out: torch.Tensor, interleaved: bool = False, rows: tuple[torch.Tensor, int] | None = None) -> None:
     """``out[n, i] = silu(gate_i) * up_i`` computed in float.  Columns of ``gate_up [N, 2I]``:
-    all gates then all ups, or (``interleaved``) alternating in blocks of 8."""
+    all gates then all ups, or (``interleaved``) alternating in blocks of 8.  ``out`` has the type of ``gate_up``, or
+    is bfloat16 of float gates and ups.  ``rows``: (int32 ids ``[N]``, count): only the rows with an id from 0 to count - 1, the others of ``out``
+    stay; in bfloat16.  The last two take ``I`` a multiple of 8 and tensors at multiples of 16 bytes."""
     s = _suffix(gate_up.dtype)
     _need(gate_up, None, "gate_up")
-    _need(out, gate_up.dtype, "out")
+    narrow = gate_up.dtype == torch.float32 and out.dtype == torch.bfloat16
+    _need(out, torch.bfloat16 if narrow else gate_up.dtype, "out")
     n, i2 = gate_up.shape
     if out.shape[0] != n or out.shape[1] * 2 != i2:
         raise ValueError("silu_mul: shapes do not agree")
     if interleaved and out.shape[1] % GATE_UP_BLOCK:
         raise ValueError("silu_mul: interleaved layout needs a multiple of 8")
-    name = f"kvf_silu_mul_{s}"
-    _check(_fn(name)(_ptr(gate_up), _ptr(out), n, out.shape[1], GATE_UP_BLOCK if interleaved else 0, _stream()), name)
+    block = GATE_UP_BLOCK if interleaved else 0
+    if narrow or rows is not None:
+        if out.shape[1] % 8 or gate_up.data_ptr() % 16 or out.data_ptr() % 16:
+            raise ValueError("silu_mul: float gates and ups with a bfloat16 result, and single rows, need a multiple of 8 and multiples of 16 bytes")
+    if rows is not None:
+        ids, count = rows
+        _need(ids, torch.int32, "rows")
+        if gate_up.dtype != torch.bfloat16 or ids.numel() != n:
+            raise ValueError("silu_mul: single rows are bfloat16, with one id each")
+        name = "kvf_silu_mul_of_rows"
+        _check(_fn(name)(_ptr(gate_up), _ptr(out), n, out.shape[1], block, _ptr(ids), count, _stream()), name)
+        return
+    name = "kvf_silu_mul_float_bf16" if narrow else f"kvf_silu_mul_{s}"
+    _check(_fn(name)(_ptr(gate_up), _ptr(out), n, out.shape[1], block, _stream()), name)
 
 
 def cast_from_float(src: torch.Tensor, out: torch.Tensor) -> None:
@@ -1084,12 +1102,14 @@ def tcgen05_ok(x: torch.Tensor, w: torch.Tensor, min_tiles: int = TCGEN05_MIN_TI
 
 
 def gemm_tcgen05(
-    x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, mode: str = "plain", err: torch.Tensor | None = None, bias: torch.Tensor | None = None
-) -> None:
+    x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, mode: str = "plain", err: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+    apart: tuple[torch.Tensor, int, torch.Tensor] | None = None,
+) -> None:  # fmt: skip
     """``x [M, K] @ w [N, K]^T`` in bfloat16 on the tcgen05 tensor cores (TMA loads, float
     accumulation in tensor memory).  ``out``: bfloat16 ``[M, N]``, or with ``mode="silu"``
     bfloat16 ``[M, N/2] = silu(gate) * up`` for ``w`` in the interleaved gate/up layout, or with ``mode="gelu_tanh"``
-    ``gelu_tanh(x w^T + bias)`` (``bias`` float ``[N]`` or ``None``)."""
+    ``gelu_tanh(x w^T + bias)`` (``bias`` float ``[N]`` or ``None``).  ``apart`` (with ``mode="silu"``): (int32 ids ``[M]``, count, bfloat16 ``[M, N]``): the
+    rows with an id from 0 to count - 1 go as the product leaves them to that tensor, and their rows of ``out`` stay."""
     if not tcgen05_ok(x, w, min_tiles=0):
         raise ValueError("gemm_tcgen05: needs bfloat16, K % 8 == 0, unit inner strides, 16-byte aligned rows")
     m, k = x.shape
@@ -1108,6 +1128,17 @@ def gemm_tcgen05(
             raise ValueError("gemm_tcgen05: out shape")
         code = 8 if mode == "gelu_tanh" else 0
     _check_bias(bias, n, mode)
+    if apart is not None:
+        ids, count, rows = apart
+        _need(ids, torch.int32, "apart ids")
+        _need(rows, torch.bfloat16, "apart rows", contiguous=False)
+        if mode != "silu" or ids.numel() != m or tuple(rows.shape) != (m, n) or rows.stride(1) != 1 or rows.stride(0) % 8 or rows.data_ptr() % 16:
+            raise ValueError("gemm_tcgen05: rows apart go with mode silu, one id each, to [M, N] with unit inner stride and 16-byte aligned rows")
+        name = "kvf_gemm_silu_apart_bf16"
+        _check(
+            _fn(name)(_ptr(x), _ptr(w), _ptr(out), m, n, k, x.stride(0), w.stride(0), out.stride(0), _ptr(ids), count, _ptr(rows), rows.stride(0), _ptr(err), _stream()), name
+        )
+        return
     name = "kvf_gemm_tcgen05_bf16"
     _check(_fn(name)(_ptr(x), _ptr(w), _ptr(out), m, n, k, x.stride(0), w.stride(0), out.stride(0), code, _ptr(bias), _ptr(err), _stream()), name)
 

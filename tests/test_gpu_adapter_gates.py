@@ -64,3 +64,55 @@ def test_gates_and_ups_of_many_rows_do_not_leave_the_own_kernel(monkeypatch):
     monkeypatch.setattr(ops, "linear", lambda a, w, out: (taken.append(w.data_ptr()), plain(a, w, out)))
     run(ops, rt, part, x, ids)
     assert part.w_gate_up.data_ptr() not in taken
+
+
+@pytest.mark.parametrize("hidden,inter,n", [(256, 1024, 1), (256, 1024, 3), (256, 1024, 16), (512, 4096, 600), (512, 8192, 260), (72, 400, 90)])
+def test_rows_without_an_adapter_are_what_they_are_alone(hidden, inter, n):
+    """Bit for bit, whoever the neighbours are: a few rows, many, and those of the library product."""
+    ops, rt, part, _, _, x, ids = feed_forward(hidden, inter, 16, n)
+    act, out = run(ops, rt, part, x, None)
+    got_act, got_out = run(ops, rt, part, x, ids)
+    none = (ids < 0).nonzero()[:, 0]
+    same = torch.equal(got_act[none], act[none]), torch.equal(got_out[none], out[none])
+    assert same == (True, True)
+    beyond = torch.where(ids < 0, torch.full_like(ids, 2), ids)  # ids outside the bank are none (and are reported)
+    with pytest.raises(RuntimeError, match="adapter outside the bank"):
+        run(ops, rt, part, x, beyond)
+    assert torch.equal(rt.buf("mlp.act", n, inter), got_act)
+
+
+@pytest.mark.parametrize("hidden,inter,rank,n", [(256, 1024, 16, 7), (256, 1024, 40, 16), (512, 4096, 16, 600), (512, 8192, 24, 260), (512, 4096, 128, 531)])
+def test_gates_and_ups_are_rounded_once(hidden, inter, rank, n):
+    """What gates and ups are joined to, against 64 bits.  It is rounded to bfloat16 once, and so are, of many rows with an adapter, a gate and an
+    up as they leave the product and again with the adapter added (a rounding is off by 2^-8 of the value: eight significant bits).  A gate and an up are
+    sums in 32 bits: no chain of more than 64 roundings, 2^-18 of the absolute terms; the numbers between an adapter's products are exact to 2^-18 where 32
+    bits come out and to 2^-17 else.  The exponential and the quotient of a gate of at most 16 are off by 2^-18 of themselves; the activation grows by 1.1 of a
+    gate's error at most."""
+    ops, rt, part, weights, lora, x, ids = feed_forward(hidden, inter, rank, n)
+    few = n <= ops.SKINNY_USE_M
+    assert few or ops.tcgen05_ok(x, part.w_gate_up)
+    act, _ = run(ops, rt, part, x, ids)
+    xd = x.double()
+    half = torch.finfo(torch.bfloat16).eps / 2
+    sums, errors = [], []
+    for proj in ("gate_proj", "up_proj"):
+        w = weights[f"{proj}.weight"].double()
+        s, m = xd @ w.t(), xd.abs() @ w.t().abs()
+        off = torch.zeros_like(s) if few else (ids >= 0).double()[:, None] * half * s.abs()
+        for slot, made in enumerate(lora):
+            a, b = (made[f"mlp.{proj}.lora_{k}.weight"].double() for k in "AB")
+            own = (ids == slot).double()[:, None]
+            s += own * 0.75 * ((xd @ a.t()) @ b.t())
+            m += own * 0.75 * ((xd.abs() @ a.t().abs()) @ b.t().abs())
+        if not few:
+            off += (ids >= 0).double()[:, None] * half * s.abs()
+        sums.append(s)
+        errors.append(off * (1 + 2 * half) + 2.0**-16 * m)
+    (gate, up), (eg, eu) = sums, errors
+    assert float(gate.abs().max()) < 16
+    silu = gate * torch.sigmoid(gate)
+    want = silu * up
+    before = 1.1 * eg * (up.abs() + eu) + silu.abs() * eu + 2.0**-18 * want.abs()
+    bound = before + half * (want.abs() + before) + 2.0**-30
+    off = float(((act.double() - want).abs() / bound).max())
+    assert off <= 1.0
