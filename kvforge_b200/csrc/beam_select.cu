@@ -9,8 +9,10 @@
 // The K highest are found without a sort: every warp's m-th highest thread maximum (m = K / 8 rounded up) has at least K numbers of the CTA
 // at or above the least of the eight, a bound that rises as the walk goes on and that a few dozen numbers of a stretch pass; those are
 // gathered, and each counts the ones above it.  Where too many pass (rows of one value), the K highest are taken one after another.
-// Measured: 512 rows of 128,256 logits (64 prompts of eight beams, K = 16) 57 us, 4.6 TB/s, bound by the instructions of the walk (some 13 a
-// logit and warp); four rows 9.4 us, of which the walk is 1.5, the choice 1, the ticket 1, the join 3 and the launch the rest.
+// Measured: 512 rows of 128,256 logits (64 prompts of eight beams, K = 16) 56 us, 4.7 TB/s.  No unit is full: 14 instructions a logit and warp
+// take 43 % of the issue slots, DRAM is busy half of the time; of the 12.2 cycles between two instructions of a warp 3.7 go to logits on their
+// way, 3.0 to instructions before it, and the 512 CTAs leave every seventh of the 592 places empty.  Four rows 9.4 us, of which the walk is 1.5,
+// the choice 1, the ticket 1, the join 3 and the launch the rest.
 // Order is decided in 64 bits (a logit with its place; a score in double with its place), so equal numbers never depend on which
 // thread comes first; sums of sixteen exponentials are in float, all that joins them is in double and in one order.
 #include "common.cuh"
@@ -229,7 +231,7 @@ __device__ __forceinline__ void load_batch(float (&v)[E], const float* x, int fi
 struct Walk {
   float high = -INFINITY;  // the thread's highest logit
   float m = -INFINITY;     // the warp's
-  float s = 0.f;           // the thread's sum of exponentials below m
+  double s = 0.;           // the thread's sum of exponentials below m
 };
 
 template <bool VEC>
@@ -251,7 +253,7 @@ __device__ __forceinline__ void walk_batch(Walk& t, const float (&v)[E], int at,
       if (v[e] >= least) put<false>(Cand{pack(v[e], place<VEC>(at, e)), 0}, sh);
   }
   if (wm > t.m) {
-    t.s *= ex2((t.m - wm) * L2E);
+    t.s *= (double)ex2((t.m - wm) * L2E);
     t.m = wm;
   }
   const float below = t.m > -INFINITY ? -t.m : 0.f;
@@ -266,7 +268,7 @@ __device__ __forceinline__ void walk_batch(Walk& t, const float (&v)[E], int at,
   }
   float a, b;
   apart(part, a, b);
-  t.s += a + b;
+  t.s += (double)(a + b);
 }
 
 // VEC: rows begin at multiples of 16 bytes, four logits a load.  All rows of a call are dealt out to threads alike, so that equal rows have

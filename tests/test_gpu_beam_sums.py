@@ -2,8 +2,6 @@
 
 from __future__ import annotations
 
-import math
-
 import pytest
 import torch
 
@@ -29,5 +27,6 @@ def test_small_exponentials_are_not_lost_beside_large_ones(rows, v):
     best = torch.full((rows, 2), 7.0, device="cuda")
     ops.beam_select(logits, scores, parents, tokens, best, ops.beam_workspace(rows, v, 2, "cuda"))
     want = scores.double()[:, None] - lse
-    assert (parents == 0).all() and tokens.tolist() == [[0, 1]] * rows
-    assert ((best.double() - want).abs() <= want.abs() * 2.0**-24 + 2.0**-20).all(), float((best.double() - want).abs().max()) / math.ulp(1.0)
+    assert bool((parents == 0).all()) and tokens.tolist() == [[0, 1]] * rows
+    off = float(((best.double() - want).abs() - want.abs() * 2.0**-24).max())
+    assert off <= 2.0**-20
