@@ -298,10 +298,6 @@ class BlockManager:
         return []
 
     # ------------------------------------------------------------------ sharing
-    def fork_demand(self, num_tokens: int) -> int:
-        """Pages of a group that a fork of a request with ``num_tokens`` computed tokens takes."""
-        return 1 if num_tokens % self.block_size else 0
-
     def fork(self, seq_id: str, child_id: str, num_tokens: int) -> list[tuple[int, int, int, int]]:
         """A second request with the first ``num_tokens`` tokens of ``seq_id``: full pages are shared, the page that is
         partly filled is one of the child's own.  Returns the copies to make before either writes again: (group,
