@@ -47,6 +47,10 @@ def read_adapter(source: str | Path) -> tuple[dict[str, torch.Tensor], float]:
     for f in files:
         tensors.update({name: f.tensor(name).clone() for name in f.keys()})
         f.close()
+    # the scale is for rank r: of another rank they belong to another configuration
+    for name, t in tensors.items():
+        if name.endswith(".lora_A.weight") and t.dim() == 2 and t.shape[0] != r:
+            raise AdapterError(f"{path}: {name} has rank {t.shape[0]}, the configuration says {r}")
     return tensors, scale
 
 
