@@ -65,7 +65,8 @@ class SchedulerConfig:
 @dataclass
 class AdapterConfig:
     """Room for low-rank adapters that requests name (``InferenceEngine.load_adapter``): how many are loaded at a time, and the
-    highest rank of one.  Not in umarhassan-cloud/kvforge."""
+    highest rank of one (what steps with adapters cost goes by it, not by the rank of those that are loaded: no higher than needed).
+    Not in umarhassan-cloud/kvforge."""
 
     max_adapters: int = 8
     max_rank: int = 16

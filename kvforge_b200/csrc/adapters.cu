@@ -5,7 +5,9 @@
 //
 // What bounds it is bytes (about a rank's flops a byte of x and of the rows) and, for few rows, latency.  The numbers between the two
 // products ("inner" numbers) are sums in 32 bits; bfloat16 multiplies them as two bfloat16 numbers (2^-17 of each is lost beside a result that
-// is rounded to 2^-8), or as three where the result is float.  float32 stays on the FP32 pipes.  A row's sums come in one order whatever
+// is rounded to 2^-8), or as three where the result is float.  float32 stays on the FP32 pipes, and is bound by latency too (515 rows on three
+// adapters, rank 16, 2048 -> 2048: 16.4 us, of which the sort is 4; the pipes are busy 9 % of the time, issue slots 18 %, and a warp waits most for x
+// and A, which come straight into registers).  A row's sums come in one order whatever
 // else is in the step: partial sums of k meet in shared memory and are added warp by warp and CTA by CTA.
 //
 // Few rows (and float32), one launch (`adapter_tile_kernel`): 16 rows of one adapter go to a cluster of eight CTAs.  Each warp multiplies blocks of
@@ -742,7 +744,8 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) adapt
 // result): 32 rows and a stripe of columns a CTA, 256 columns at a time.  A warp of its own fetches what the pieces need (the rows by TMA, 32
 // that follow one another a box or four gathered; the columns' rows of B are one stretch), several pieces ahead; eight warps multiply, add
 // and write 32 columns each.  What is on its way is in shared memory, not in registers.  Bound by its products and by their operands' way from
-// shared memory: 1,057 rows on 24 adapters of rank 64, 28672 columns (238 MB), some 115 us.
+// shared memory: a call of 1,057 rows on 24 adapters of rank 128, 28672 columns alternating (356 MB with both products' reads) 309 us; of 2,048 rows on
+// two, rank 128, 4096 -> 6144 in three sections 172.
 constexpr int PIECE = 256;  // columns
 constexpr int ROWS = 32;
 constexpr int MAX_STAGES = 4;
@@ -1264,8 +1267,8 @@ int run_wide(AdapterParams p, const Maps& maps, int tiles, cudaStream_t st) {
     return launch(kernel, dim3(SMS), dim3(32 * (ADDERS + FETCHERS + 1)), held + stages * fed, st, p, outer, tiles, stages);
   }
 
-  // Two CTAs an SM where few inner numbers stay in registers (2,048 float rows on eight adapters, 4096 columns of rank 32: 42 us so, 63 with one CTA and
-  // more numbers; 2,048 of rank 64: 91 and 81).
+  // Float results of two sections and more: two CTAs an SM where few inner numbers stay in registers (2,048 rows on eight adapters, two sections of 2048
+  // columns: rank 16 34 us so and 56 with one CTA and more numbers, rank 32 46 and 64; 28672 columns alternating, rank 32: 227 and 284).
   const bool few_ranks = sizeof(O) == 4 && p.R <= 32;
   const int places = few_ranks ? 2 : 1;
   const size_t stage = (size_t)PIECE * sizeof(O) * ROWS + (size_t)PIECE * p.R * 2;

@@ -2884,7 +2884,9 @@ class AdapterBank:
     or bfloat16), ``scales`` float ``[S]``.  Adapter ``s`` adds ``scales[s] * b[s] (a[s] x)`` to the projection's result; a section is one of the
     matrices that are stacked in the projection and has rows of ``a`` of its own.  ``ends``: the column after each section's last;
     ``alternating``: two sections whose columns alternate in blocks of 8 (``interleave_gate_up``).  ``R`` is a multiple of 16: ranks
-    below it are filled with zeros; ``ranks`` (int32 ``[S]``) says how many rows of each section are not."""
+    below it are filled with zeros; ``ranks`` (int32 ``[S]``) says how many rows of each section are not.  Those rows alone are multiplied and fetched of
+    ``a``, but most kernels fetch ``b`` all ``R`` wide, and which of them run goes by ``R``: a bank for a higher rank than its adapters have costs
+    time."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, ends=None, alternating: bool = False, ranks: torch.Tensor | None = None) -> None:
         _suffix(a.dtype)
@@ -2925,7 +2927,7 @@ class AdapterBank:
 ADAPTER_DIRECT = 64  # up to so many rows the kernels group for themselves
 # from so many bfloat16 rows on the two products are kernels of their own: 32 clusters of 16 rows find room at the same time (one adapter of rank
 # 16, 4096 x 6144: 512 rows 16 us in one kernel and 22 in two, 600 rows 24 and 24; 4096 x 28672: 29 and 30, 49 and 34; 20 of rank 64 there: 116 and
-# 88, 119 and 98)
+# 88, 119 and 98: the rule goes by rows alone, so that many adapters of a high rank just below it are slower than they would be above it)
 ADAPTER_MANY = 513
 ADAPTER_TILE = 128  # rows of one adapter that a tile of the list has room for
 
